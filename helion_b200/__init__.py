@@ -3,6 +3,8 @@
 Public surface:
     fp8_gemm, fp8_attention         -- operators on torch CUDA tensors (helion_b200.ops)
     preprocess_fp8_attention_inputs -- q, k, v -> e4m3 in one kernel, with the reference's views
+    rms_norm_quantize               -- RMS norm with the residual's addition, 8-bit codes and row scales out
+    quantize_rows                   -- 16- / 32-bit rows -> 8-bit codes (e4m3 or int8) and row scales
     HostGemm                        -- fp8_gemm on pinned host buffers with overlapped PCIe copies
     matmul                          -- fp16 / bf16 sibling of fp8_gemm with the bias / ReLU epilogues
     attention                       -- fp16 / bf16 sibling of fp8_attention (examples/attention.py)
@@ -14,13 +16,24 @@ from __future__ import annotations
 
 from ._lib import DeviceWaitTimeout, LibraryNotBuiltError
 from .host_io import HostGemm
-from .ops import attention, attention_into, fp8_attention, fp8_gemm, matmul, preprocess_fp8_attention_inputs
+from .ops import (
+    attention,
+    attention_into,
+    fp8_attention,
+    fp8_gemm,
+    matmul,
+    preprocess_fp8_attention_inputs,
+    quantize_rows,
+    rms_norm_quantize,
+)
 
 __all__ = [
     "fp8_gemm",
     "fp8_attention",
     "attention_into",
     "preprocess_fp8_attention_inputs",
+    "rms_norm_quantize",
+    "quantize_rows",
     "HostGemm",
     "matmul",
     "attention",

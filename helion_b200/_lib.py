@@ -24,7 +24,7 @@ ERR_TIMEOUT = -7
 ERR_BAD_CONFIG = -8
 ERR_WORKSPACE = -9
 
-DT_FP16, DT_BF16, DT_FP32, DT_E4M3 = 0, 1, 2, 3
+DT_FP16, DT_BF16, DT_FP32, DT_E4M3, DT_INT8 = 0, 1, 2, 3, 4
 OP_GEMM, OP_ATTENTION = 0, 1
 STATIC_SCRATCH_BYTES = 4 << 20
 ATTN_WORKSPACE_BYTES = 16
@@ -74,6 +74,15 @@ SIGNATURES = {
     "hb200_fp8_attention_preprocess": (
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _i64, ctypes.c_int, ctypes.c_int, _vp],
+    ),
+    "hb200_quantize_rows": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp],
+    ),
+    "hb200_rms_norm_quantize": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+         ctypes.c_float, ctypes.c_int, _vp],
     ),
     "hb200_fp8_attention_ws": (
         ctypes.c_int,

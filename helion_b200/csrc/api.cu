@@ -483,6 +483,62 @@ int hb200_gemm_16bit(const void* x, const void* y, void* out, int64_t M, int64_t
   return launch_gemm_16bit(a, ctx);
 }
 
+// Validation and launch shared by the two row-quantisation entry points.
+static int row_quantize_impl(const char* what, const RowQuantCall& c, int device, void* stream) {
+  const std::string name(what);
+  if (c.src_dtype != HB200_DT_FP16 && c.src_dtype != HB200_DT_BF16 && c.src_dtype != HB200_DT_FP32) {
+    return set_error(HB200_ERR_BAD_DTYPE, name + ": src_dtype must be FP16, BF16 or FP32");
+  }
+  if (c.out_dtype != HB200_DT_E4M3 && c.out_dtype != HB200_DT_INT8) {
+    return set_error(HB200_ERR_BAD_DTYPE, name + ": out_dtype must be E4M3 or INT8");
+  }
+  if (c.weight_dtype != c.src_dtype && c.weight_dtype != HB200_DT_FP32) {
+    return set_error(HB200_ERR_BAD_DTYPE, name + ": weight_dtype must be src_dtype or FP32");
+  }
+  if (c.M < 1 || c.N < 1 || c.M > INT32_MAX || c.N > INT32_MAX) {
+    return set_error(HB200_ERR_BAD_SHAPE, name + ": M and N must be in [1, 2^31)");
+  }
+  if (c.x == nullptr || c.codes == nullptr || c.scales == nullptr) return set_error(HB200_ERR_ALIGN, name + ": null pointer");
+  if ((c.residual == nullptr) != (c.residual_out == nullptr)) {
+    return set_error(HB200_ERR_ALIGN, name + ": residual and residual_out go together");
+  }
+  if (c.x_rs < c.N || c.codes_rs < c.N || (c.residual != nullptr && (c.residual_rs < c.N || c.residual_out_rs < c.N))) {
+    return set_error(HB200_ERR_BAD_STRIDE, name + ": row strides must be >= N");
+  }
+  const uintptr_t elem = c.src_dtype == HB200_DT_FP32 ? 4 : 2;
+  const uintptr_t w_elem = c.weight_dtype == HB200_DT_FP32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.residual) |
+       reinterpret_cast<uintptr_t>(c.residual_out)) % elem != 0 ||
+      reinterpret_cast<uintptr_t>(c.weight) % w_elem != 0 || reinterpret_cast<uintptr_t>(c.scales) % 4 != 0) {
+    return set_error(HB200_ERR_ALIGN, name + ": pointers must be aligned to their element size");
+  }
+  // an eps that is zero in fp32 would leave a row whose squares underflow without a finite root
+  if (c.weight != nullptr && !(c.eps >= 1.17549435e-38f && c.eps <= 3.402823466e38f)) {
+    return set_error(HB200_ERR_BAD_CONFIG, name + ": eps must be a positive normal fp32 number");
+  }
+  DeviceCtx* ctx = get_device_ctx(device);
+  if (ctx == nullptr) return ctx_error_code(device);
+  HB_DEVICE_GUARD(device);
+  return launch_row_quantize(c, static_cast<cudaStream_t>(stream));
+}
+
+int hb200_quantize_rows(const void* x, void* codes, float* scales, int64_t M, int64_t N, int64_t x_rs, int64_t codes_rs,
+                        int src_dtype, int out_dtype, int device, void* stream) {
+  const RowQuantCall c{x, nullptr, nullptr, codes, scales, nullptr, M, N, x_rs, 0, codes_rs, 0, src_dtype, src_dtype,
+                       out_dtype, 0.0f};
+  return row_quantize_impl("quantize_rows", c, device, stream);
+}
+
+int hb200_rms_norm_quantize(const void* x, const void* residual, const void* weight, void* codes, float* scales,
+                            void* residual_out, int64_t M, int64_t N, int64_t x_rs, int64_t residual_rs, int64_t codes_rs,
+                            int64_t residual_out_rs, int src_dtype, int weight_dtype, int out_dtype, float eps, int device,
+                            void* stream) {
+  if (weight == nullptr) return set_error(HB200_ERR_ALIGN, "rms_norm_quantize: null pointer");
+  const RowQuantCall c{x, residual, weight, codes, scales, residual_out, M, N, x_rs, residual_rs, codes_rs,
+                       residual_out_rs, src_dtype, weight_dtype, out_dtype, eps};
+  return row_quantize_impl("rms_norm_quantize", c, device, stream);
+}
+
 int hb200_fp8_gemm_splitk_static(const void* x, const void* y, void* out, int64_t M, int64_t N, int64_t K,
                                  int64_t x_rs, int64_t x_cs, int64_t y_rs, int64_t y_cs, int64_t out_rs, int out_dtype,
                                  int splits, int device, void* stream) {

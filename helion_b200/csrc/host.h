@@ -161,6 +161,19 @@ int launch_attention_16bit(const AttnArgs& args, DeviceCtx* ctx);
 // q, k, v (fp16 / bf16 / fp32, `count` elements each) -> e4m3fn with torch's cast rule (quantize.cu).
 int launch_attention_preprocess(const void* q, const void* k, const void* v, void* q8, void* k8, void* v8, int64_t count,
                                 int src_dtype, DeviceCtx* ctx, cudaStream_t stream);
+// Row-wise quantisation, alone (weight null) or behind an RMS norm with the residual's addition (row_quantize.cu).
+struct RowQuantCall {
+  const void* x;
+  const void* residual;  // null: none
+  const void* weight;    // null: no norm
+  void* codes;
+  float* scales;
+  void* residual_out;
+  int64_t M, N, x_rs, residual_rs, codes_rs, residual_out_rs;
+  int src_dtype, weight_dtype, out_dtype;
+  float eps;
+};
+int launch_row_quantize(const RowQuantCall& c, cudaStream_t stream);
 // The two-tile attention kernel (fp8_attention_pair.cu) on tensor maps built for 128-key steps; non-causal only.
 int launch_fp8_attention_pair(const AttnArgs& args, DeviceCtx* ctx, const CUtensorMap& tq, const CUtensorMap& tk,
                               const CUtensorMap& tv, bool v_kmajor, int poly_of8, bool lazy);

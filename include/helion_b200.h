@@ -51,6 +51,7 @@ extern "C" {
 #define HB200_DT_BF16 1
 #define HB200_DT_FP32 2
 #define HB200_DT_E4M3 3
+#define HB200_DT_INT8 4 /* 8-bit codes of the row-wise quantisation and operands of the int8 GEMMs */
 
 /* operations (for the tile-config queries) */
 #define HB200_OP_GEMM 0
@@ -196,6 +197,33 @@ HB200_API int hb200_attention_16bit(const void* q, const void* k, const void* v,
  * 16-byte aligned device pointers. */
 HB200_API int hb200_fp8_attention_preprocess(const void* q, const void* k, const void* v, void* q8, void* k8, void* v8,
                                    int64_t count, int src_dtype, int device, void* stream);
+
+/* Row-wise quantisation to 8 bits: for each row of x [M,N] one scale and N codes,
+ *   scale = max(max|x| / Q, FLT_MIN),  code = round_to_nearest_even(x / scale),  Q = 448 (E4M3) or 127 (INT8),
+ * in fp32.  The codes and scales are what hb200_fp8_gemm_scaled / hb200_int8_gemm take as x and scale_a with
+ * HB200_SCALE_ROWWISE.  The reference has no counterpart (its fp8 example casts without scales,
+ * examples/fp8_gemm.py:60-75).
+ *   x: src_dtype FP16, BF16 or FP32, row stride x_rs >= N elements, aligned to its element size;
+ *   codes: E4M3 or INT8 bytes, row stride codes_rs >= N;  scales: M floats;  N >= 1, any M >= 1.
+ * Aligned rows (16 bytes, N a multiple of 8) and rows that all start at the same place modulo 8 elements are read
+ * with wide loads; other layouts element by element.
+ * A row whose max|x| is below 2^-100 gets codes of zero and the scale FLT_MIN.  A NaN in a row makes its scale NaN;
+ * an infinity makes it infinite. */
+HB200_API int hb200_quantize_rows(const void* x, void* codes, float* scales, int64_t M, int64_t N, int64_t x_rs,
+                                  int64_t codes_rs, int src_dtype, int out_dtype, int device, void* stream);
+
+/* hb200_quantize_rows behind a root-mean-square norm with the residual's addition, in one pass:
+ *   s = x + residual;  y = s / sqrt(mean(s^2) + eps) * weight;  codes and scales of y;  residual_out = cast(s).
+ * The norm takes the fp32 sum s before it is rounded to src_dtype for residual_out.
+ *   residual: NULL (s = x; residual_out must then be NULL too), else [M,N] of src_dtype;
+ *   residual_out: [M,N] of src_dtype; may be x or residual itself (same pointer and stride), no other overlap;
+ *   weight: N values, weight_dtype = src_dtype or FP32.  eps: a positive normal fp32 number.
+ * A row whose max|s * weight| is below 2^-100, or whose scale would be below FLT_MIN, gets codes of zero and the
+ * scale FLT_MIN; a sum of squares that is not finite in fp32 makes the row's scale NaN. */
+HB200_API int hb200_rms_norm_quantize(const void* x, const void* residual, const void* weight, void* codes, float* scales,
+                                      void* residual_out, int64_t M, int64_t N, int64_t x_rs, int64_t residual_rs,
+                                      int64_t codes_rs, int64_t residual_out_rs, int src_dtype, int weight_dtype,
+                                      int out_dtype, float eps, int device, void* stream);
 
 /* Split-K FP8 GEMM that allocates nothing: same computation and arguments as hb200_fp8_gemm with a
  * split-K row of the table, but the fp32 partial sums live in a fixed array compiled into the
