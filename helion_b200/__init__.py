@@ -3,6 +3,7 @@
 Public surface:
     fp8_gemm, fp8_attention         -- operators on torch CUDA tensors (helion_b200.ops)
     preprocess_fp8_attention_inputs -- q, k, v -> e4m3 in one kernel, with the reference's views
+    int8_gemm                       -- int8 sibling of fp8_gemm (scales for each token and channel)
     rms_norm_quantize               -- RMS norm with the residual's addition, 8-bit codes and row scales out
     quantize_rows                   -- 16- / 32-bit rows -> 8-bit codes (e4m3 or int8) and row scales
     HostGemm                        -- fp8_gemm on pinned host buffers with overlapped PCIe copies
@@ -21,6 +22,7 @@ from .ops import (
     attention_into,
     fp8_attention,
     fp8_gemm,
+    int8_gemm,
     matmul,
     preprocess_fp8_attention_inputs,
     quantize_rows,
@@ -32,6 +34,7 @@ __all__ = [
     "fp8_attention",
     "attention_into",
     "preprocess_fp8_attention_inputs",
+    "int8_gemm",
     "rms_norm_quantize",
     "quantize_rows",
     "HostGemm",

@@ -416,6 +416,69 @@ int hb200_fp8_gemm_scaled(const void* x, const void* y, void* out, int64_t M, in
                        cfg_id, workspace, workspace_bytes, device, stream);
 }
 
+int hb200_int8_gemm(const void* x, const void* y, void* out, int64_t M, int64_t N, int64_t K, int64_t x_rs, int64_t x_cs,
+                    int64_t y_rs, int64_t y_cs, int64_t out_rs, int out_dtype, const float* scale_a, const float* scale_b,
+                    int scale_mode, int cfg_id, int device, void* stream) {
+  if (scale_mode != HB200_SCALE_NONE && scale_mode != HB200_SCALE_TENSOR && scale_mode != HB200_SCALE_ROWWISE) {
+    return set_error(HB200_ERR_BAD_CONFIG, "int8_gemm: scale_mode must be HB200_SCALE_NONE, _TENSOR or _ROWWISE");
+  }
+  if (scale_mode != HB200_SCALE_NONE) {
+    if (scale_a == nullptr || scale_b == nullptr) return set_error(HB200_ERR_ALIGN, "int8_gemm: null scale pointer");
+    if ((reinterpret_cast<uintptr_t>(scale_a) | reinterpret_cast<uintptr_t>(scale_b)) & 3u) {
+      return set_error(HB200_ERR_ALIGN, "int8_gemm: scale pointers must be 4-byte aligned");
+    }
+  }
+  if (out_dtype != HB200_DT_FP16 && out_dtype != HB200_DT_BF16 && out_dtype != HB200_DT_FP32) {
+    return set_error(HB200_ERR_BAD_DTYPE, "int8_gemm: out_dtype must be FP16, BF16 or FP32");
+  }
+  if (M < 1 || N < 1 || K < 1 || M > INT32_MAX || N > INT32_MAX) {
+    return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: M and N must be in [1, 2^31), K positive");
+  }
+  if (K >= 131072) return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: K must be below 131072 (the sums are int32)");
+  if (K % 16 != 0) return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: K must be a multiple of 16");
+  if (N % 8 != 0) return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: N must be a multiple of 8");
+  if (x == nullptr || y == nullptr || out == nullptr) return set_error(HB200_ERR_ALIGN, "int8_gemm: null pointer");
+  if (x_cs != 1) return set_error(HB200_ERR_BAD_STRIDE, "int8_gemm: x must be row-major (column stride 1)");
+  if (x_rs < K || x_rs % 16 != 0) {
+    return set_error(HB200_ERR_BAD_STRIDE, "int8_gemm: x row stride must be >= K and a multiple of 16");
+  }
+  if (y_rs != 1 || y_cs < K || y_cs % 16 != 0) {
+    return set_error(HB200_ERR_BAD_STRIDE, "int8_gemm: y must be column-major (row stride 1), its column stride >= K and a multiple of 16");
+  }
+  const int64_t out_elem = out_dtype == HB200_DT_FP32 ? 4 : 2;
+  if (out_rs < N || (out_rs * out_elem) % 16 != 0) {
+    return set_error(HB200_ERR_BAD_STRIDE, "int8_gemm: out row stride must be >= N and give 16-byte aligned rows");
+  }
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) & 15u) {
+    return set_error(HB200_ERR_ALIGN, "int8_gemm: x, y and out must be 16-byte aligned");
+  }
+  DeviceCtx* ctx = get_device_ctx(device);
+  if (ctx == nullptr) return ctx_error_code(device);
+  GemmArgs a;
+  a.x = x;
+  a.y = y;
+  a.out = out;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.lda = x_rs;
+  a.ldb = y_cs;
+  a.y_colmajor = true;
+  a.ldc = out_rs;
+  a.out_dtype = out_dtype;
+  a.cfg_id = cfg_id;
+  a.workspace = nullptr;
+  a.workspace_bytes = 0;
+  a.device = device;
+  a.stream = static_cast<cudaStream_t>(stream);
+  a.scale_a = scale_a;
+  a.scale_b = scale_b;
+  a.scale_mode = scale_mode;
+  a.kind = KIND_S8;
+  HB_DEVICE_GUARD(device);
+  return launch_int8_gemm(a, ctx);
+}
+
 int hb200_gemm_16bit(const void* x, const void* y, void* out, int64_t M, int64_t N, int64_t K, int64_t x_rs, int64_t x_cs,
                      int64_t y_rs, int64_t y_cs, int64_t out_rs, int in_dtype, int out_dtype, const float* bias, int relu,
                      int cfg_id, int device, void* stream) {

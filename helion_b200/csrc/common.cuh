@@ -25,9 +25,10 @@ namespace hb {
 constexpr unsigned long long HB_WAIT_LIMIT_NS = 2000000000ull;  // 2 s per wait
 constexpr unsigned long long HB_DRAIN_LIMIT_NS = 200000000ull;  // 0.2 s per drain wait
 
-// Operand kinds of the GEMM kernels: e4m3 (kind::f8f6f4) or 16-bit floats (kind::f16).  All of them
-// move 32 bytes of K per instruction, so the byte-oriented pipelines are shared.
-enum OperandKind : int { KIND_E4M3 = 0, KIND_F16 = 1, KIND_BF16 = 2 };
+// Operand kinds of the GEMM kernels: e4m3 (kind::f8f6f4), 16-bit floats (kind::f16) or signed 8-bit integers
+// (kind::i8).  All of them move 32 bytes of K per instruction, so the byte-oriented pipelines are shared.
+enum OperandKind : int { KIND_E4M3 = 0, KIND_F16 = 1, KIND_BF16 = 2, KIND_S8 = 3 };
+__host__ __device__ constexpr int kind_bytes(int kind) { return kind == KIND_F16 || kind == KIND_BF16 ? 2 : 1; }
 
 enum WaitSite : uint32_t {
   SITE_GEMM_EMPTY = 1,
@@ -310,10 +311,24 @@ __device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, ui
       : "memory");
 }
 
+// Same for signed 8-bit integers (int32 accumulator, wrapping), K = 32 elements.
+__device__ __forceinline__ void umma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 template <int KIND>
 __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                         uint32_t accumulate) {
   if constexpr (KIND == KIND_E4M3) umma_f8_ss(d_tmem, a_desc, b_desc, idesc, accumulate);
+  else if constexpr (KIND == KIND_S8) umma_i8_ss(d_tmem, a_desc, b_desc, idesc, accumulate);
   else umma_f16_ss(d_tmem, a_desc, b_desc, idesc, accumulate);
 }
 
@@ -465,10 +480,23 @@ __device__ __forceinline__ void umma_f16_ss_pair(uint32_t d_tmem, uint64_t a_des
       : "memory");
 }
 
+__device__ __forceinline__ void umma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 template <int KIND>
 __device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                              uint32_t accumulate) {
   if constexpr (KIND == KIND_E4M3) umma_f8_ss_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
+  else if constexpr (KIND == KIND_S8) umma_i8_ss_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
   else umma_f16_ss_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
 }
 
@@ -517,12 +545,13 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(uint32_t m, uint32_t n, b
          ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-// Instruction descriptor for any of the kinds above (fp32 accumulator).  kind::f16 encodes f16 as
-// format 0 and bf16 as format 1 in the same A / B format fields.
+// Instruction descriptor for any of the kinds above.  kind::f16 encodes f16 as format 0 and bf16 as format 1 in the
+// same A / B format fields, kind::i8 encodes signed operands as format 1.  Accumulator format: 1 = f32, 2 = s32.
 template <int KIND>
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t m, uint32_t n, bool a_mn_major, bool b_mn_major) {
-  constexpr uint32_t fmt = KIND == KIND_BF16 ? 1u : 0u;
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
+  constexpr uint32_t fmt = KIND == KIND_BF16 || KIND == KIND_S8 ? 1u : 0u;
+  constexpr uint32_t acc = KIND == KIND_S8 ? 2u : 1u;
+  return (acc << 4) | (fmt << 7) | (fmt << 10) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
          ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 

@@ -64,6 +64,15 @@ __device__ __forceinline__ void scales_only_chunk(uint32_t (&r)[32], const EpiSc
   }
 }
 
+// kind::i8 accumulators are int32: to fp32, one rounding where a sum needs more than 24 bits.
+template <int KIND>
+__device__ __forceinline__ void acc_to_float(uint32_t (&r)[32]) {
+  if constexpr (KIND == KIND_S8) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__int2float_rn(static_cast<int>(r[i])));
+  }
+}
+
 // The whole epilogue on one chunk: scales, then bias, then ReLU.  (Kept free of recursion and of copies
 // of `r`, so that the 32 values stay in registers.)
 __device__ __forceinline__ void scale_chunk(uint32_t (&r)[32], const EpiScale& sc, int row, int M, int col0, int N) {

@@ -163,7 +163,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   // splits > 1: split-K.  Work unit u = (tile u % num_tiles, K range u / num_tiles); every unit writes
   // its fp32 partial tile to partials[split][M][N] and splitk_reduce_kernel sums and converts.
   using L = GemmLayout<BN, STAGES>;
-  constexpr int ES = KIND == KIND_E4M3 ? 1 : 2;  // element size of x and y
+  constexpr int ES = kind_bytes(KIND);  // element size of x and y
   constexpr int KROWS = BK / ES;                 // K rows of an MN-major B stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -333,6 +333,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           if (splits > 1) {
             store_row_chunk<HB200_DT_FP32>(part, 0, col0, N, r);  // unscaled; the reduce pass scales
           } else {
+            acc_to_float<KIND>(r);
             scale_chunk(r, sc, row, M, col0, N);
             store_row_chunk<OUT_DT>(out, row_off, col0, N, r);
           }
@@ -425,7 +426,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
                      const __grid_constant__ CUtensorMap tmap_out, int M, int N, int K, int group_m, uint32_t* status,
                      EpiScale sc) {
   using L = PairLayout<STAGES>;
-  constexpr int ES = KIND == KIND_E4M3 ? 1 : 2;
+  constexpr int ES = kind_bytes(KIND);
   constexpr int KROWS = BK / ES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -594,6 +595,7 @@ fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         tmem_ld_32x32b_x32(t_row + c, r);
         tmem_wait_ld();
         const int col = tc.n_blk * PAIR_BN + c;
+        acc_to_float<KIND>(r);
         scale_chunk(r, sc, row0 + lane, M, col, N);
         StagedStore<OUT_DT>::store(r, stage, chunk_count, lane, &tmap_out, col, row0, row0 < M && col < N);
       }
@@ -680,9 +682,9 @@ fp8_gemm_pair2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                       const __grid_constant__ CUtensorMap tmap_out, int M, int N, int K, int group_m,
                       uint32_t* status, EpiScale sc) {
   using L = Pair2Layout<STAGES, PAIR2_BN>;
-  static_assert(PAIR2_BN == 256 || (PAIR2_BN == 224 && !B_MN_MAJOR && KIND == KIND_E4M3), "tile widths built");
+  static_assert(PAIR2_BN == 256 || (PAIR2_BN == 224 && !B_MN_MAJOR && kind_bytes(KIND) == 1), "tile widths built");
   static_assert(L::STAGE_BYTES % 1024 == 0 && 2 * PAIR2_BN <= L::TMEM_COLS, "swizzle alignment / tensor memory");
-  constexpr int ES = KIND == KIND_E4M3 ? 1 : 2;
+  constexpr int ES = kind_bytes(KIND);
   constexpr int KROWS = BK / ES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -870,6 +872,7 @@ fp8_gemm_pair2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         tmem_ld_32x32b_x32(t_row + c, r);
         tmem_wait_ld();
         const int col = tc.n_blk * PAIR2_BN + c;
+        acc_to_float<KIND>(r);
         scale_chunk(r, sc, row0 + lane, M, col, N);
 #ifdef HB_GEMM_TRACE
         const bool tr = threadIdx.x == 64 && tile_iter == 0 && c < 256;
@@ -971,7 +974,7 @@ int encode_out_map(CUtensorMap* tout, const GemmArgs& a) {
 // K as the kernels see it: the byte length of a row of x.
 template <int KIND>
 int k_bytes(const GemmArgs& a) {
-  return static_cast<int>(a.K * (KIND == KIND_E4M3 ? 1 : 2));
+  return static_cast<int>(a.K * kind_bytes(KIND));
 }
 
 template <int STAGES, bool B_MN, int OUT_DT, int KIND = KIND_E4M3>
@@ -1448,6 +1451,61 @@ int launch_gemm_16bit(const GemmArgs& a, DeviceCtx* ctx) {
     return set_error(HB200_ERR_BAD_DTYPE, "gemm_16bit: bf16 operands give a BF16 or FP32 result");
   }
   return set_error(HB200_ERR_BAD_DTYPE, "gemm_16bit: operands must be FP16 or BF16");
+}
+
+// ------------------------------------------------------------------------------------------------
+// Signed 8-bit integer operands through the same kernels (hb200_int8_gemm): kind::i8 instructions, int32
+// accumulators, y column-major.  The tensor pipe runs them at the e4m3 rate, so the table and its choice are the
+// same; up to 128 rows of x go to the weight-streaming kernel instead (gemm_few_rows.cu).
+// ------------------------------------------------------------------------------------------------
+namespace {
+
+template <int OUT_DT>
+int launch_s8_row(const GemmArgs& a, DeviceCtx* ctx, const GemmConfig& c, const CUtensorMap& ta, const CUtensorMap& tb) {
+  if (c.pair && c.bn == 448) return launch_pair2_instance<false, OUT_DT, KIND_S8, 224>(a, ctx, ta, tb, c.group_m);
+  if (c.pair && c.bn == 512) return launch_pair2_instance<false, OUT_DT, KIND_S8>(a, ctx, ta, tb, c.group_m);
+  if (c.pair) return launch_pair_instance<6, false, OUT_DT, KIND_S8>(a, ctx, ta, tb, c.group_m);
+  if (c.bn == 256) return launch_instance<256, 4, false, OUT_DT, KIND_S8>(a, ctx, ta, tb, c.group_m);
+  if (c.bn == 128) return launch_instance<128, 6, false, OUT_DT, KIND_S8>(a, ctx, ta, tb, c.group_m);
+  return launch_instance<64, 8, false, OUT_DT, KIND_S8>(a, ctx, ta, tb, c.group_m);
+}
+
+}  // namespace
+
+int launch_int8_gemm(const GemmArgs& a, DeviceCtx* ctx) {
+  int cfg_id = a.cfg_id;
+  if (cfg_id < 0) {
+    if (a.M <= kFewRowsMax) return launch_few_rows(few_rows_args(a), ctx);
+    cfg_id = gemm_select_config_nosplit(a.M, a.N, a.K, true, ctx->num_sms);
+  }
+  if (cfg_id >= kNumGemmConfigs) return set_error(HB200_ERR_BAD_CONFIG, "int8_gemm: no such config");
+  const GemmConfig& c = kGemmConfigs[cfg_id];
+  if (c.splits > 1 || c.skinny_mode != 0) {
+    return set_error(HB200_ERR_BAD_CONFIG, "int8_gemm: this table row exists for e4m3 operands only");
+  }
+  if (c.skinny) {
+    if (a.M > kFewRowsMax) return set_error(HB200_ERR_BAD_CONFIG, "int8_gemm: this row takes at most 128 rows of x");
+    return launch_few_rows(few_rows_args(a), ctx);
+  }
+  CUtensorMap ta, tb;
+  const uint64_t dims_a[2] = {static_cast<uint64_t>(a.K), static_cast<uint64_t>(a.M)};
+  const uint64_t strides_a[1] = {static_cast<uint64_t>(a.lda)};
+  const uint32_t box_a[2] = {BK, static_cast<uint32_t>(is_pair2(c) ? 256 : BM)};
+  int rc = encode_tmap_u8(&ta, a.x, 2, dims_a, strides_a, box_a, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != HB200_OK) return rc;
+  const uint64_t dims_b[2] = {static_cast<uint64_t>(a.K), static_cast<uint64_t>(a.N)};
+  const uint64_t strides_b[1] = {static_cast<uint64_t>(a.ldb)};
+  const uint32_t box_b[2] = {BK, static_cast<uint32_t>(is_pair2(c) ? pair2_width(c) / 2 : (c.pair ? 128 : c.bn))};
+  rc = encode_tmap_u8(&tb, a.y, 2, dims_b, strides_b, box_b, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != HB200_OK) return rc;
+  switch (a.out_dtype) {
+    case HB200_DT_FP16:
+      return launch_s8_row<HB200_DT_FP16>(a, ctx, c, ta, tb);
+    case HB200_DT_BF16:
+      return launch_s8_row<HB200_DT_BF16>(a, ctx, c, ta, tb);
+    default:
+      return launch_s8_row<HB200_DT_FP32>(a, ctx, c, ta, tb);
+  }
 }
 
 }  // namespace hb

@@ -108,7 +108,7 @@ struct GemmArgs {
   const float* scale_a = nullptr;
   const float* scale_b = nullptr;
   int scale_mode = 0;
-  // 16-bit operands (hb200_gemm_16bit): 0 = e4m3, 1 = fp16, 2 = bf16; optional bias / ReLU epilogue
+  // operands (OperandKind): 0 = e4m3, 1 = fp16, 2 = bf16, 3 = int8; optional bias / ReLU epilogue (16-bit)
   int kind = 0;
   const float* bias = nullptr;
   int relu = 0;
@@ -117,6 +117,30 @@ struct GemmArgs {
 int launch_fp8_gemm(const GemmArgs& args, DeviceCtx* ctx);
 // Same kernels with fp16 / bf16 operands (args.kind); M, N, K and strides in elements.
 int launch_gemm_16bit(const GemmArgs& args, DeviceCtx* ctx);
+// Same kernels with signed 8-bit integer operands (column-major y).
+int launch_int8_gemm(const GemmArgs& args, DeviceCtx* ctx);
+
+// Up to 128 rows of x against one weight (int8) or the two weights of a gated projection, all column-major
+// (gemm_few_rows.cu).
+constexpr int64_t kFewRowsMax = 128;
+struct FewRowsArgs {
+  const void* x = nullptr;
+  const void* w[2] = {nullptr, nullptr};
+  void* out = nullptr;
+  int64_t M = 0, N = 0, K = 0;
+  int64_t lda = 0, ldb[2] = {0, 0}, ldc = 0;
+  int out_dtype = 0;
+  int kind = 0;        // OperandKind
+  bool gated = false;  // out = act(x w[0]) * (x w[1])
+  int act = 0;         // Activation
+  int device = 0;
+  cudaStream_t stream = nullptr;
+  const float* scale_x = nullptr;
+  const float* scale_w[2] = {nullptr, nullptr};
+  int scale_mode = 0;
+};
+FewRowsArgs few_rows_args(const GemmArgs& args);
+int launch_few_rows(const FewRowsArgs& args, DeviceCtx* ctx);
 int gemm_num_configs();
 int gemm_describe_config(int cfg_id, char* buf, int buf_len);
 int gemm_select_config(int64_t M, int64_t N, int64_t K, bool y_colmajor, int out_dtype, int num_sms);

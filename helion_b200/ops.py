@@ -161,23 +161,84 @@ def fp8_gemm(
     return out
 
 
-def _check_scales(scale_a, scale_b, m: int, n: int, device):
+def _check_scales(scale_a, scale_b, m: int, n: int, device, what: str = "fp8_gemm"):
     """Validate the two scale tensors; returns contiguous fp32 tensors and the C-ABI scale mode."""
     if scale_a is None or scale_b is None:
-        raise ValueError("fp8_gemm: pass both scale_a and scale_b or neither")
+        raise ValueError(f"{what}: pass both scale_a and scale_b or neither")
     for name, t in (("scale_a", scale_a), ("scale_b", scale_b)):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
-            raise TypeError(f"fp8_gemm: {name} must be a float32 tensor")
+            raise TypeError(f"{what}: {name} must be a float32 tensor")
         if t.device != device:
-            raise ValueError(f"fp8_gemm: {name} must live on the inputs' device")
+            raise ValueError(f"{what}: {name} must live on the inputs' device")
     if scale_a.numel() == 1 and scale_b.numel() == 1:
         return scale_a.reshape(1).contiguous(), scale_b.reshape(1).contiguous(), _lib.SCALE_TENSOR
     if tuple(scale_a.shape) in ((m, 1), (m,)) and tuple(scale_b.shape) in ((1, n), (n,)):
         return scale_a.reshape(m).contiguous(), scale_b.reshape(n).contiguous(), _lib.SCALE_ROWWISE
     raise ValueError(
-        f"fp8_gemm: scales must be one element each, or [M,1]/[M] and [1,N]/[N]; got {tuple(scale_a.shape)} and "
+        f"{what}: scales must be one element each, or [M,1]/[M] and [1,N]/[N]; got {tuple(scale_a.shape)} and "
         f"{tuple(scale_b.shape)} for M={m}, N={n}"
     )
+
+
+def int8_gemm(
+    x: torch.Tensor,
+    y: torch.Tensor,
+    *,
+    scale_a: Optional[torch.Tensor] = None,
+    scale_b: Optional[torch.Tensor] = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    config: Optional[int] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``out = (((x @ y) * scale_a) * scale_b).to(out_dtype)`` for int8 ``x [M,K]`` and ``y [K,N]``: exact integer sums.
+
+    The int8 sibling of :func:`fp8_gemm` with its arguments: ``scale_a`` / ``scale_b`` (fp32, both or neither) are one
+    element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of ``y`` (``[1, N]`` / ``[N]``), as
+    :func:`quantize_rows` and :func:`rms_norm_quantize` make them.  ``y`` is best column-major (a transposed view of
+    ``[N, K]`` storage); a row-major one is re-laid out in every call.  ``K`` is below 131072.
+    """
+    if x.dtype != torch.int8 or y.dtype != torch.int8:
+        raise TypeError(f"int8_gemm expects int8 inputs, got {x.dtype} and {y.dtype}")
+    if x.dim() != 2 or y.dim() != 2:
+        raise ValueError(f"int8_gemm expects 2-D inputs, got {tuple(x.shape)} and {tuple(y.shape)}")
+    m, k = x.shape
+    k2, n = y.shape
+    assert k == k2, f"size mismatch {k} != {k2}"
+    if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"int8_gemm out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
+    dev = _require_cuda(x, y)
+    sa_ptr = sb_ptr = None
+    mode = _lib.SCALE_NONE
+    if scale_a is not None or scale_b is not None:
+        scale_a, scale_b, mode = _check_scales(scale_a, scale_b, m, n, x.device, "int8_gemm")
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    elif out.dtype != out_dtype or tuple(out.shape) != (m, n) or out.stride(1) != 1 or out.device != x.device:
+        raise ValueError("int8_gemm: `out` must be a row-major [M, N] tensor of out_dtype on the inputs' device")
+    if m == 0 or n == 0:
+        return out
+    if k == 0:
+        return out.zero_()
+    if k % 16 != 0 or n % 8 != 0:  # odd K or N: the same kernels on zero-padded copies (see _pad_gemm_operands)
+        np_ = _round_up(n, 16)
+        y = y if y.stride(0) == 1 else y.t().contiguous().t()
+        xp, yp = _pad_gemm_operands(x, y, _round_up(k, 16), np_)
+        if mode == _lib.SCALE_ROWWISE:
+            scale_b = _pad_vector(scale_b, n, np_, 1.0)
+        out.copy_(int8_gemm(xp, yp, scale_a=scale_a if mode else None, scale_b=scale_b if mode else None, out_dtype=out_dtype, config=config)[:, :n])
+        return out
+    if x.stride(1) != 1 or x.stride(0) % 16 != 0 or x.stride(0) < k or x.data_ptr() % 16 != 0:
+        x = x.clone(memory_format=torch.contiguous_format)
+    if y.stride(0) != 1 or y.stride(1) % 16 != 0 or y.stride(1) < k or y.data_ptr() % 16 != 0:
+        y = y.t().clone(memory_format=torch.contiguous_format).t()
+    if mode != _lib.SCALE_NONE:
+        sa_ptr, sb_ptr = scale_a.data_ptr(), scale_b.data_ptr()
+    code = _lib.load().hb200_int8_gemm(
+        x.data_ptr(), y.data_ptr(), out.data_ptr(), m, n, k, x.stride(0), 1, 1, y.stride(1), out.stride(0),
+        _OUT_DT[out_dtype], sa_ptr, sb_ptr, mode, -1 if config is None else int(config), dev, _stream_ptr(dev),
+    )
+    _lib.raise_for(code, "int8_gemm")
+    return out
 
 
 def _kernel_head_dim(d: int, what: str) -> int:

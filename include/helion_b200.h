@@ -96,6 +96,19 @@ HB200_API int hb200_fp8_gemm_scaled(const void* x, const void* y, void* out, int
                           const float* scale_a, const float* scale_b, int scale_mode, int cfg_id, void* workspace,
                           size_t workspace_bytes, int device, void* stream);
 
+/* out = cast(((x @ y) * scale_a) * scale_b) for int8 x [M,K] and y [K,N]: the integer sums are exact (int32), then
+ * one conversion to fp32 and the two fp32 multiplications of hb200_fp8_gemm_scaled.  The int8 sibling of the fp8 GEMM
+ * (examples/fp8_gemm.py:29-57); the reference has none.
+ *   x: int8, row-major, x_rs % 16 == 0;  y: int8, column-major (y_rs == 1), y_cs % 16 == 0; both 16-byte aligned.
+ *   K % 16 == 0, K < 131072 (so that no sum leaves int32);  N % 8 == 0;  out: FP16 / BF16 / FP32, rows 16-byte aligned.
+ *   scale_mode HB200_SCALE_NONE (scale_a and scale_b are not read), _TENSOR or _ROWWISE.
+ *   cfg_id: -1, or a row of the GEMM table without split-K and chain forms (0-10, 14-18, 21); -1 and row 18 run up to
+ *   128 rows of x in a kernel of their own that streams y. */
+HB200_API int hb200_int8_gemm(const void* x, const void* y, void* out, int64_t M, int64_t N, int64_t K, int64_t x_rs,
+                              int64_t x_cs, int64_t y_rs, int64_t y_cs, int64_t out_rs, int out_dtype,
+                              const float* scale_a, const float* scale_b, int scale_mode, int cfg_id, int device,
+                              void* stream);
+
 /* out = cast(epilogue(x @ y)) for fp16 or bf16 x [M,K] and y [K,N] with fp32 accumulation: the same
  * kernels with kind::f16 tensor-core instructions.  Replaces the device kernel of the reference's
  * examples/matmul.py:26-56 (`matmul(x, y, epilogue)`; zero-initialised fp32 accumulator, torch.addmm
