@@ -6,6 +6,8 @@ Public surface:
     int8_gemm                       -- int8 sibling of fp8_gemm (scales for each token and channel)
     rms_norm_quantize               -- RMS norm with the residual's addition, 8-bit codes and row scales out
     quantize_rows                   -- 16- / 32-bit rows -> 8-bit codes (e4m3 or int8) and row scales
+    gated_matmul                    -- act(x Wg) * (x Wu) in one kernel, fp16 / bf16 with gradients
+    gated_gemm                      -- the same with e4m3 / int8 operands and scales
     HostGemm                        -- fp8_gemm on pinned host buffers with overlapped PCIe copies
     matmul                          -- fp16 / bf16 sibling of fp8_gemm with the bias / ReLU epilogues
     attention                       -- fp16 / bf16 sibling of fp8_attention (examples/attention.py)
@@ -16,6 +18,7 @@ There is no CPU, Triton or PyTorch fallback: calls fail loudly when the CUDA lib
 from __future__ import annotations
 
 from ._lib import DeviceWaitTimeout, LibraryNotBuiltError
+from .gated import gated_gemm, gated_matmul
 from .host_io import HostGemm
 from .ops import (
     attention,
@@ -37,6 +40,8 @@ __all__ = [
     "int8_gemm",
     "rms_norm_quantize",
     "quantize_rows",
+    "gated_matmul",
+    "gated_gemm",
     "HostGemm",
     "matmul",
     "attention",

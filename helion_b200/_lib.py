@@ -29,6 +29,7 @@ OP_GEMM, OP_ATTENTION = 0, 1
 STATIC_SCRATCH_BYTES = 4 << 20
 ATTN_WORKSPACE_BYTES = 16
 SCALE_NONE, SCALE_TENSOR, SCALE_ROWWISE = 0, 1, 2
+ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2
 
 # Every symbol the header declares, with (restype, argtypes).
 _i64 = ctypes.c_int64
@@ -79,6 +80,16 @@ SIGNATURES = {
     "hb200_fp8_attention_preprocess": (
         ctypes.c_int,
         [_vp, _vp, _vp, _vp, _vp, _vp, _i64, ctypes.c_int, ctypes.c_int, _vp],
+    ),
+    "hb200_gated_gemm": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+         _vp, _vp, _vp, ctypes.c_int, _vp, _vp, ctypes.c_int, _vp],
+    ),
+    "hb200_gated_gemm_backward": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int,
+         _vp, ctypes.c_size_t, ctypes.c_int, _vp],
     ),
     "hb200_quantize_rows": (
         ctypes.c_int,

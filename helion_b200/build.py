@@ -23,7 +23,7 @@ OUT_DIR = PKG_DIR / "_C"
 LIB_PATH = OUT_DIR / "libhelion_b200.so"
 INCLUDE_DIR = PKG_DIR.parent / "include"
 
-SOURCES = ["api.cu", "fp8_gemm.cu", "fp8_gemm_skinny.cu", "fp8_attention.cu", "fp8_attention_pair.cu", "softmax_ceiling.cu", "attention_16bit.cu", "quantize.cu", "row_quantize.cu", "gemm_few_rows.cu"]
+SOURCES = ["api.cu", "fp8_gemm.cu", "fp8_gemm_skinny.cu", "fp8_attention.cu", "fp8_attention_pair.cu", "softmax_ceiling.cu", "attention_16bit.cu", "quantize.cu", "row_quantize.cu", "gemm_few_rows.cu", "gated_forward.cu", "gated_backward.cu"]
 
 NVCC_FLAGS = [
     "-gencode",

@@ -546,6 +546,167 @@ int hb200_gemm_16bit(const void* x, const void* y, void* out, int64_t M, int64_t
   return launch_gemm_16bit(a, ctx);
 }
 
+// Layout and limits shared by the gated projection and its gradients.  w_colmajor receives the weights' layout.
+static int gated_check(const char* what, int64_t M, int64_t F, int64_t K, int64_t x_rs, int64_t gate_rs, int64_t gate_cs,
+                       int64_t up_rs, int64_t up_cs, int in_dtype, bool* w_colmajor, int64_t ldb[2]) {
+  const std::string name(what);
+  const int64_t per16 = in_dtype == HB200_DT_FP16 || in_dtype == HB200_DT_BF16 ? 8 : 16;  // elements in 16 bytes
+  if (M < 1 || F < 1 || K < 1 || M > INT32_MAX || F > INT32_MAX / 2 || K > INT32_MAX / 4) {
+    return set_error(HB200_ERR_BAD_SHAPE, name + ": M must be in [1, 2^31), F in [1, 2^30), K in [1, 2^29)");
+  }
+  if (K % per16 != 0) return set_error(HB200_ERR_BAD_SHAPE, name + ": K must be a multiple of 16 bytes");
+  if (F % 8 != 0) return set_error(HB200_ERR_BAD_SHAPE, name + ": F must be a multiple of 8");
+  if (x_rs < K || x_rs % per16 != 0) {
+    return set_error(HB200_ERR_BAD_STRIDE, name + ": rows of x must be >= K long and 16-byte aligned");
+  }
+  const bool col = gate_rs == 1 && up_rs == 1 && gate_cs >= K && up_cs >= K;
+  const bool row = gate_cs == 1 && up_cs == 1 && gate_rs >= F && up_rs >= F && per16 == 8;
+  if (!col && !row) {
+    return set_error(HB200_ERR_BAD_STRIDE, name + ": both weights must be column-major (row stride 1) or, with 16-bit "
+                                                  "operands, both row-major (column stride 1)");
+  }
+  *w_colmajor = col;
+  ldb[0] = col ? gate_cs : gate_rs;
+  ldb[1] = col ? up_cs : up_rs;
+  if (ldb[0] % per16 != 0 || ldb[1] % per16 != 0) {
+    return set_error(HB200_ERR_BAD_STRIDE, name + ": the weights' leading strides must be multiples of 16 bytes");
+  }
+  return HB200_OK;
+}
+
+int hb200_gated_gemm(const void* x, const void* w_gate, const void* w_up, void* out, int64_t M, int64_t F, int64_t K,
+                     int64_t x_rs, int64_t gate_rs, int64_t gate_cs, int64_t up_rs, int64_t up_cs, int64_t out_rs, int in_dtype,
+                     int out_dtype, int act, const float* scale_x, const float* scale_gate, const float* scale_up,
+                     int scale_mode, float* saved_p, float* saved_a, int device, void* stream) {
+  const bool half = in_dtype == HB200_DT_FP16 || in_dtype == HB200_DT_BF16;
+  if (!half && in_dtype != HB200_DT_E4M3 && in_dtype != HB200_DT_INT8) {
+    return set_error(HB200_ERR_BAD_DTYPE, "gated_gemm: in_dtype must be FP16, BF16, E4M3 or INT8");
+  }
+  if (half ? out_dtype != in_dtype : (out_dtype != HB200_DT_FP16 && out_dtype != HB200_DT_BF16 && out_dtype != HB200_DT_FP32)) {
+    return set_error(HB200_ERR_BAD_DTYPE, "gated_gemm: out_dtype must be the 16-bit operands' type, or FP16, BF16 or FP32 for 8-bit ones");
+  }
+  if (act != HB200_ACT_SILU && act != HB200_ACT_GELU && act != HB200_ACT_GELU_TANH) {
+    return set_error(HB200_ERR_BAD_CONFIG, "gated_gemm: unknown activation");
+  }
+  if (scale_mode != HB200_SCALE_NONE && scale_mode != HB200_SCALE_TENSOR && scale_mode != HB200_SCALE_ROWWISE) {
+    return set_error(HB200_ERR_BAD_CONFIG, "gated_gemm: scale_mode must be HB200_SCALE_NONE, _TENSOR or _ROWWISE");
+  }
+  if (half && scale_mode != HB200_SCALE_NONE) return set_error(HB200_ERR_BAD_CONFIG, "gated_gemm: scales are for 8-bit operands");
+  if ((saved_p == nullptr) != (saved_a == nullptr) || (saved_p != nullptr && !half)) {
+    return set_error(HB200_ERR_BAD_CONFIG, "gated_gemm: saved_p and saved_a go together, with 16-bit operands");
+  }
+  bool w_colmajor = true;
+  int64_t ldb[2] = {0, 0};
+  const int rc = gated_check("gated_gemm", M, F, K, x_rs, gate_rs, gate_cs, up_rs, up_cs, in_dtype, &w_colmajor, ldb);
+  if (rc != HB200_OK) return rc;
+  if (in_dtype == HB200_DT_INT8 && K >= 131072) {
+    return set_error(HB200_ERR_BAD_SHAPE, "gated_gemm: K must be below 131072 for int8 operands (the sums are int32)");
+  }
+  const int64_t out_elem = out_dtype == HB200_DT_FP32 ? 4 : 2;
+  if (out_rs < F || (out_rs * out_elem) % 16 != 0) {
+    return set_error(HB200_ERR_BAD_STRIDE, "gated_gemm: out row stride must be >= F and give 16-byte aligned rows");
+  }
+  if (x == nullptr || w_gate == nullptr || w_up == nullptr || out == nullptr) return set_error(HB200_ERR_ALIGN, "gated_gemm: null pointer");
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w_gate) | reinterpret_cast<uintptr_t>(w_up) |
+       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(saved_p) | reinterpret_cast<uintptr_t>(saved_a)) & 15u) {
+    return set_error(HB200_ERR_ALIGN, "gated_gemm: pointers must be 16-byte aligned");
+  }
+  if (scale_mode != HB200_SCALE_NONE) {
+    if (scale_x == nullptr || scale_gate == nullptr || scale_up == nullptr) {
+      return set_error(HB200_ERR_ALIGN, "gated_gemm: null scale pointer");
+    }
+    if ((reinterpret_cast<uintptr_t>(scale_x) | reinterpret_cast<uintptr_t>(scale_gate) | reinterpret_cast<uintptr_t>(scale_up)) & 3u) {
+      return set_error(HB200_ERR_ALIGN, "gated_gemm: scale pointers must be 4-byte aligned");
+    }
+  }
+  DeviceCtx* ctx = get_device_ctx(device);
+  if (ctx == nullptr) return ctx_error_code(device);
+  GatedArgs a;
+  a.x = x;
+  a.w[0] = w_gate;
+  a.w[1] = w_up;
+  a.out = out;
+  a.saved[0] = saved_p;
+  a.saved[1] = saved_a;
+  a.M = M;
+  a.F = F;
+  a.K = K;
+  a.lda = x_rs;
+  a.ldb[0] = ldb[0];
+  a.ldb[1] = ldb[1];
+  a.ldc = out_rs;
+  a.w_colmajor = w_colmajor;
+  a.kind = in_dtype == HB200_DT_FP16 ? KIND_F16 : (in_dtype == HB200_DT_BF16 ? KIND_BF16 : (in_dtype == HB200_DT_INT8 ? KIND_S8 : KIND_E4M3));
+  a.out_dtype = out_dtype;
+  a.act = act;
+  a.scale_x = scale_x;
+  a.scale_w[0] = scale_gate;
+  a.scale_w[1] = scale_up;
+  a.scale_mode = scale_mode;
+  a.device = device;
+  a.stream = static_cast<cudaStream_t>(stream);
+  HB_DEVICE_GUARD(device);
+  return launch_gated(a, ctx);
+}
+
+int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const float* saved_p,
+                              const float* saved_a, void* dx, void* dw_gate, void* dw_up, int64_t M, int64_t F, int64_t K,
+                              int64_t dh_rs, int64_t x_rs, int64_t gate_rs, int64_t gate_cs, int64_t up_rs, int64_t up_cs,
+                              int dtype, void* workspace, size_t workspace_bytes, int device, void* stream) {
+  if (dtype != HB200_DT_FP16 && dtype != HB200_DT_BF16) {
+    return set_error(HB200_ERR_BAD_DTYPE, "gated_gemm_backward: dtype must be FP16 or BF16");
+  }
+  bool w_colmajor = true;
+  int64_t ldb[2] = {0, 0};
+  const int rc = gated_check("gated_gemm_backward", M, F, K, x_rs, gate_rs, gate_cs, up_rs, up_cs, dtype, &w_colmajor, ldb);
+  if (rc != HB200_OK) return rc;
+  if (dh_rs < F || dh_rs % 8 != 0) {
+    return set_error(HB200_ERR_BAD_STRIDE, "gated_gemm_backward: rows of dh must be >= F long and 16-byte aligned");
+  }
+  if (dh == nullptr || x == nullptr || w_gate == nullptr || w_up == nullptr || saved_p == nullptr || saved_a == nullptr) {
+    return set_error(HB200_ERR_ALIGN, "gated_gemm_backward: null pointer");
+  }
+  if ((dw_gate == nullptr) != (dw_up == nullptr)) {
+    return set_error(HB200_ERR_ALIGN, "gated_gemm_backward: dw_gate and dw_up go together");
+  }
+  if ((reinterpret_cast<uintptr_t>(dh) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w_gate) |
+       reinterpret_cast<uintptr_t>(w_up) | reinterpret_cast<uintptr_t>(saved_p) | reinterpret_cast<uintptr_t>(saved_a) |
+       reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw_gate) | reinterpret_cast<uintptr_t>(dw_up)) & 15u) {
+    return set_error(HB200_ERR_ALIGN, "gated_gemm_backward: pointers must be 16-byte aligned");
+  }
+  // 4*M*F bytes against the workspace, by division: the product of the sizes cannot wrap that way
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
+      static_cast<uint64_t>(M) > workspace_bytes / (4u * static_cast<uint64_t>(F))) {
+    return set_error(HB200_ERR_WORKSPACE, "gated_gemm_backward: needs a 16-byte aligned workspace of 2*M*F 16-bit values");
+  }
+  DeviceCtx* ctx = get_device_ctx(device);
+  if (ctx == nullptr) return ctx_error_code(device);
+  GatedGradArgs a;
+  a.dh = dh;
+  a.x = x;
+  a.w[0] = w_gate;
+  a.w[1] = w_up;
+  a.saved[0] = saved_p;
+  a.saved[1] = saved_a;
+  a.dx = dx;
+  a.dw[0] = dw_gate;
+  a.dw[1] = dw_up;
+  a.dgu = workspace;
+  a.M = M;
+  a.F = F;
+  a.K = K;
+  a.dh_rs = dh_rs;
+  a.lda = x_rs;
+  a.ldb[0] = ldb[0];
+  a.ldb[1] = ldb[1];
+  a.w_colmajor = w_colmajor;
+  a.kind = dtype == HB200_DT_FP16 ? KIND_F16 : KIND_BF16;
+  a.device = device;
+  a.stream = static_cast<cudaStream_t>(stream);
+  HB_DEVICE_GUARD(device);
+  return launch_gated_grad(a, ctx);
+}
+
 // Validation and launch shared by the two row-quantisation entry points.
 static int row_quantize_impl(const char* what, const RowQuantCall& c, int device, void* stream) {
   const std::string name(what);

@@ -141,6 +141,41 @@ struct FewRowsArgs {
 };
 FewRowsArgs few_rows_args(const GemmArgs& args);
 int launch_few_rows(const FewRowsArgs& args, DeviceCtx* ctx);
+// The gated projection out = act(x w[0]) * (x w[1]) (gated_forward.cu) and its gradients (gated_backward.cu).
+struct GatedArgs {
+  const void* x = nullptr;
+  const void* w[2] = {nullptr, nullptr};  // gate, up
+  void* out = nullptr;
+  float* saved[2] = {nullptr, nullptr};   // P = u act'(g) and A = act(g), [M,F] each; null: not kept
+  int64_t M = 0, F = 0, K = 0;
+  int64_t lda = 0, ldb[2] = {0, 0}, ldc = 0;
+  bool w_colmajor = true;
+  int kind = 0;  // OperandKind
+  int out_dtype = 0;
+  int act = 0;   // Activation
+  const float* scale_x = nullptr;
+  const float* scale_w[2] = {nullptr, nullptr};
+  int scale_mode = 0;
+  int device = 0;
+  cudaStream_t stream = nullptr;
+};
+int launch_gated(const GatedArgs& args, DeviceCtx* ctx);
+struct GatedGradArgs {
+  const void* dh = nullptr;
+  const void* x = nullptr;
+  const void* w[2] = {nullptr, nullptr};
+  const float* saved[2] = {nullptr, nullptr};
+  void* dx = nullptr;                      // null: not wanted
+  void* dw[2] = {nullptr, nullptr};        // null: not wanted
+  void* dgu = nullptr;                     // workspace: dG and dU, [M,F] each of the operands' type
+  int64_t M = 0, F = 0, K = 0;
+  int64_t dh_rs = 0, lda = 0, ldb[2] = {0, 0};
+  bool w_colmajor = true;                  // of w, and of dw, which is contiguous in that layout
+  int kind = 0;
+  int device = 0;
+  cudaStream_t stream = nullptr;
+};
+int launch_gated_grad(const GatedGradArgs& args, DeviceCtx* ctx);
 int gemm_num_configs();
 int gemm_describe_config(int cfg_id, char* buf, int buf_len);
 int gemm_select_config(int64_t M, int64_t N, int64_t K, bool y_colmajor, int out_dtype, int num_sms);

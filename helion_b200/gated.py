@@ -1,0 +1,228 @@
+"""The gated projection of a feed-forward block: ``act(x @ w_gate) * (x @ w_up)`` in one kernel.
+
+:func:`gated_matmul` takes fp16 / bf16 operands and has gradients; :func:`gated_gemm` takes e4m3 / int8 operands with
+scales, as :func:`helion_b200.rms_norm_quantize` and :func:`helion_b200.quantize_rows` make them.  The reference's
+examples stop at one product with an epilogue (examples/matmul.py:26-56).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _OUT_DT, _require_cuda, _round_up, _stream_ptr
+
+_ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
+
+
+def _check_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str, what: str) -> int:
+    if x.dim() != 2 or w_gate.dim() != 2 or w_up.dim() != 2:
+        raise ValueError(f"{what} expects 2-D inputs, got {tuple(x.shape)}, {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    if w_gate.shape != w_up.shape:
+        raise ValueError(f"{what}: w_gate {tuple(w_gate.shape)} and w_up {tuple(w_up.shape)} differ in shape")
+    if x.shape[1] != w_gate.shape[0]:
+        raise ValueError(f"{what}: size mismatch, x is {tuple(x.shape)} and the weights {tuple(w_gate.shape)}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+    return _ACTIVATIONS[activation]
+
+
+def _rows_ready(t: torch.Tensor, per16: int) -> torch.Tensor:
+    """``t`` itself where its rows are what the kernels read (unit column stride, 16-byte aligned), else a copy."""
+    if t.stride(1) == 1 and t.stride(0) % per16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _weights_ready(w_gate: torch.Tensor, w_up: torch.Tensor, per16: int, row_major: bool):
+    """Both weights in one layout the kernels read: column-major, or row-major where that is allowed and they are."""
+    if row_major and w_gate.stride(1) == 1 and w_up.stride(1) == 1 and w_gate.stride(0) != 1 and w_up.stride(0) != 1:
+        return _rows_ready(w_gate, per16), _rows_ready(w_up, per16)
+    return _rows_ready(w_gate.t(), per16).t(), _rows_ready(w_up.t(), per16).t()
+
+
+def _launch(x, w_gate, w_up, out, act: int, scales=(None, None, None), mode: int = _lib.SCALE_NONE, saved=(None, None), what: str = "gated_gemm"):
+    dev = _require_cuda(x, w_gate, w_up, out)
+    ptr = [t.data_ptr() if t is not None else None for t in (*scales, *saved)]
+    code = _lib.load().hb200_gated_gemm(
+        x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), x.shape[0], out.shape[1], x.shape[1],
+        x.stride(0), w_gate.stride(0), w_gate.stride(1), w_up.stride(0), w_up.stride(1), out.stride(0),
+        _OUT_DT[x.dtype], _OUT_DT[out.dtype], act, *ptr[:3], mode, *ptr[3:], dev, _stream_ptr(dev),
+    )
+    _lib.raise_for(code, what)
+    return out
+
+
+class _GatedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, act):
+        x = _rows_ready(x, 8)
+        w_gate, w_up = _weights_ready(w_gate, w_up, 8, True)
+        m, f = x.shape[0], w_gate.shape[1]
+        out = torch.empty((m, f), dtype=x.dtype, device=x.device)
+        # u * act'(g) and act(g) in fp32: the gradients of g and u are then rounded once, as operands of their products
+        p, a = torch.empty((2, m, f), dtype=torch.float32, device=x.device)
+        _launch(x, w_gate, w_up, out, act, saved=(p, a), what="gated_matmul")
+        ctx.save_for_backward(x, w_gate, w_up, p, a)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        x, w_gate, w_up, p, a = ctx.saved_tensors
+        m, k = x.shape
+        f = w_gate.shape[1]
+        dev = _require_cuda(dh, x)
+        dh = _rows_ready(dh, 8)
+        dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
+        dw_gate = dw_up = None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            if w_gate.stride(0) == 1:
+                dw_gate, dw_up = (torch.empty((f, k), dtype=x.dtype, device=x.device).t() for _ in range(2))
+            else:
+                dw_gate, dw_up = (torch.empty((k, f), dtype=x.dtype, device=x.device) for _ in range(2))
+        workspace = torch.empty((2, m, f), dtype=x.dtype, device=x.device)
+        ptr = [t.data_ptr() if t is not None else None for t in (dx, dw_gate, dw_up)]
+        code = _lib.load().hb200_gated_gemm_backward(
+            dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), p.data_ptr(), a.data_ptr(), *ptr, m, f, k,
+            dh.stride(0), x.stride(0), w_gate.stride(0), w_gate.stride(1), w_up.stride(0), w_up.stride(1),
+            _OUT_DT[x.dtype], workspace.data_ptr(), workspace.numel() * workspace.element_size(), dev, _stream_ptr(dev),
+        )
+        _lib.raise_for(code, "gated_matmul backward")
+        return dx, dw_gate if ctx.needs_input_grad[1] else None, dw_up if ctx.needs_input_grad[2] else None, None
+
+
+_NODE_STREAM = "helion_b200.stream"  # key in a gradient accumulator's metadata: the stream it was first used on here
+
+
+def _accumulators(*leaves: torch.Tensor) -> list:
+    """The gradient accumulators of the leaves among ``leaves``; refuses a capture that their streams would break.
+
+    Autograd ties a leaf's accumulator to the stream it was made on for as long as any graph over that leaf lives.  A
+    backward pass under capture then waits on that stream, which CUDA forbids for the default one: the capture is lost
+    in the middle of the backward pass.  So it is refused here, before anything is recorded.
+    """
+    nodes = []
+    for t in leaves:
+        if t.requires_grad and t.grad_fn is None:
+            node = torch.autograd.graph.get_gradient_edge(t).node
+            stream = _stream_ptr(t.device.index)
+            if node.metadata.setdefault(_NODE_STREAM, stream) == 0 and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(
+                    "gated_matmul: an eager graph over the same leaf tensors, made on the default stream, is still alive; "
+                    "a backward pass cannot be captured next to it. Drop its results first, or make it on another stream"
+                )
+            nodes.append(node)
+    return nodes
+
+
+def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation: str = "silu") -> torch.Tensor:
+    """``act(x @ w_gate) * (x @ w_up)`` for fp16 or bf16 ``x [M,K]`` and weights ``[K,F]``, with gradients.
+
+    Both products, the activation (``"silu"``, ``"gelu"`` or ``"gelu_tanh"``) and the product run in one kernel with
+    fp32 accumulation; the result has the operands' dtype, rounded once.  The weights may be column-major (a transposed
+    view of ``[F, K]`` storage) or row-major, both in the same layout (else one is copied).  When a gradient is needed
+    the forward pass also keeps two fp32 ``[M,F]`` tensors; the backward pass returns ``x``'s and the weights' gradients
+    in their dtype, and is not differentiable itself.  Both passes can be captured into a CUDA graph, unless an eager
+    graph over the same leaf tensors, made on the default stream, is alive: that is refused.
+    """
+    if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"gated_matmul expects three float16 or three bfloat16 tensors, got {x.dtype}, {w_gate.dtype} and {w_up.dtype}")
+    act = _check_gated(x, w_gate, w_up, activation, "gated_matmul")
+    _require_cuda(x, w_gate, w_up)
+    m, k = x.shape
+    f = w_gate.shape[1]
+    if m == 0 or f == 0 or k == 0:
+        return (x @ w_gate) * (x @ w_up)  # without elements, or zeros: act(0) = 0
+    grad = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
+    held = _accumulators(x, w_gate, w_up) if grad else None  # noqa: F841  (alive until the graph holds them)
+    kp, fp = _round_up(k, 8), _round_up(f, 8)
+    if kp != k or fp != f:  # odd K or F: the same kernels on zero-padded copies; zero columns give act(0) * 0
+        pad = torch.nn.functional.pad
+        weights = (pad(w.t(), (0, kp - k, 0, fp - f)).t() for w in (w_gate, w_up))
+        return gated_matmul(pad(x, (0, kp - k)), *weights, activation=activation)[:, :f]
+    if grad:
+        return _GatedMatmul.apply(x, w_gate, w_up, act)
+    x = _rows_ready(x, 8)
+    w_gate, w_up = _weights_ready(w_gate, w_up, 8, True)
+    return _launch(x, w_gate, w_up, torch.empty((m, f), dtype=x.dtype, device=x.device), act, what="gated_matmul")
+
+
+def _gated_scales(scale_x, scale_gate, scale_up, m: int, f: int, device):
+    """Validate the three scales; returns contiguous fp32 vectors and the C-ABI scale mode."""
+    scales = (scale_x, scale_gate, scale_up)
+    if all(s is None for s in scales):
+        return scales, _lib.SCALE_NONE
+    if any(s is None for s in scales):
+        raise ValueError("gated_gemm: pass scale_x, scale_gate and scale_up, or none of them")
+    for name, t in zip(("scale_x", "scale_gate", "scale_up"), scales):
+        if t.dtype != torch.float32:
+            raise TypeError(f"gated_gemm: {name} must be a float32 tensor")
+        if t.device != device:
+            raise ValueError(f"gated_gemm: {name} must live on the inputs' device")
+    if all(s.numel() == 1 for s in scales):
+        return tuple(s.reshape(1) for s in scales), _lib.SCALE_TENSOR
+    if tuple(scale_x.shape) in ((m, 1), (m,)) and all(tuple(s.shape) in ((1, f), (f,)) for s in scales[1:]):
+        return tuple(s.reshape(-1).contiguous() for s in scales), _lib.SCALE_ROWWISE
+    raise ValueError(
+        "gated_gemm: scales must be one element each, or [M,1]/[M], [1,F]/[F] and [1,F]/[F]; got "
+        f"{tuple(scale_x.shape)}, {tuple(scale_gate.shape)} and {tuple(scale_up.shape)} for M={m}, F={f}"
+    )
+
+
+def gated_gemm(
+    x: torch.Tensor,
+    w_gate: torch.Tensor,
+    w_up: torch.Tensor,
+    *,
+    scale_x: Optional[torch.Tensor] = None,
+    scale_gate: Optional[torch.Tensor] = None,
+    scale_up: Optional[torch.Tensor] = None,
+    activation: str = "silu",
+    out_dtype: torch.dtype = torch.bfloat16,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``act(g) * u`` with ``g = (x @ w_gate) * scale_x * scale_gate`` and ``u`` likewise, for e4m3 or int8 operands.
+
+    ``x [M,K]`` and the weights ``[K,F]`` share one 8-bit dtype (``float8_e4m3fn`` or ``int8``).  The fp32 scales (all
+    three or none) are one element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of the
+    weights (``[1, F]`` / ``[F]``).  One kernel, ``g`` and ``u`` in fp32, one rounding to ``out_dtype`` (fp16, bf16 or
+    fp32).  Weights are best column-major (a transposed view of ``[F, K]`` storage); row-major ones are re-laid out in
+    every call.  Up to 128 rows of ``x`` run in a kernel that streams the weights.
+    """
+    if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise TypeError(f"gated_gemm expects three float8_e4m3fn or three int8 tensors, got {x.dtype}, {w_gate.dtype} and {w_up.dtype}")
+    act = _check_gated(x, w_gate, w_up, activation, "gated_gemm")
+    if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"gated_gemm out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
+    _require_cuda(x, w_gate, w_up)
+    m, k = x.shape
+    f = w_gate.shape[1]
+    scales, mode = _gated_scales(scale_x, scale_gate, scale_up, m, f, x.device)
+    if out is None:
+        out = torch.empty((m, f), dtype=out_dtype, device=x.device)
+    elif out.dtype != out_dtype or tuple(out.shape) != (m, f) or out.stride(1) != 1 or out.device != x.device:
+        raise ValueError("gated_gemm: `out` must be a row-major [M, F] tensor of out_dtype on the inputs' device")
+    if m == 0 or f == 0:
+        return out
+    if k == 0:
+        return out.zero_()
+    kp, fp = _round_up(k, 16), _round_up(f, 8)
+    if kp != k or fp != f:  # odd K or F: the same kernels on zero-padded copies
+        xp = x.new_zeros((m, kp))
+        xp[:, :k].copy_(x)
+        padded = []
+        for w in (w_gate, w_up):
+            wp = w.new_zeros((fp, kp))
+            wp[:f, :k].copy_(w.t())
+            padded.append(wp.t())
+        if mode == _lib.SCALE_ROWWISE:
+            scales = (scales[0], *(torch.nn.functional.pad(s, (0, fp - f)) for s in scales[1:]))
+        res = torch.empty((m, fp), dtype=out_dtype, device=x.device)
+        out.copy_(_launch(xp, *padded, res, act, scales, mode)[:, :f])
+        return out
+    x = _rows_ready(x, 16)
+    w_gate, w_up = _weights_ready(w_gate, w_up, 16, False)
+    return _launch(x, w_gate, w_up, out, act, scales, mode)

@@ -211,6 +211,39 @@ HB200_API int hb200_attention_16bit(const void* q, const void* k, const void* v,
 HB200_API int hb200_fp8_attention_preprocess(const void* q, const void* k, const void* v, void* q8, void* k8, void* v8,
                                    int64_t count, int src_dtype, int device, void* stream);
 
+/* The gated projection of a feed-forward block: out[M,F] = cast(act(g) * u) with g = x @ w_gate and u = x @ w_up, both
+ * products, the activation and the product in one kernel; g and u stay in fp32 (int32 for int8 operands).
+ *   in_dtype: FP16 or BF16 (out_dtype the same, no scales), or E4M3 or INT8 (out_dtype FP16, BF16 or FP32).
+ *   scale_mode (8-bit operands): HB200_SCALE_NONE; _TENSOR: g = (x @ w_gate) * scale_x[0] * scale_gate[0], u likewise;
+ *     _ROWWISE: scale_x holds M floats, scale_gate and scale_up F each.
+ *   act: HB200_ACT_SILU, HB200_ACT_GELU (with the normal distribution function) or HB200_ACT_GELU_TANH.
+ *   x: row-major, rows 16-byte aligned; w_gate, w_up [K,F]: both column-major or, 16-bit operands only, both row-major, the
+ *     other axis's stride giving 16-byte aligned rows; out: row-major, rows 16-byte aligned.
+ *   K a multiple of 16 bytes (16 or 8 elements), K < 131072 for INT8; F % 8 == 0.  Pointers 16-byte aligned.
+ *   saved_p, saved_a: NULL, or (16-bit operands) [M,F] contiguous floats each that receive u * act'(g) and act(g) for
+ *     hb200_gated_gemm_backward.
+ * The reference has no counterpart (its examples stop at one product with an epilogue, examples/matmul.py:26-56). */
+#define HB200_ACT_SILU 0
+#define HB200_ACT_GELU 1
+#define HB200_ACT_GELU_TANH 2
+HB200_API int hb200_gated_gemm(const void* x, const void* w_gate, const void* w_up, void* out, int64_t M, int64_t F, int64_t K,
+                               int64_t x_rs, int64_t gate_rs, int64_t gate_cs, int64_t up_rs, int64_t up_cs, int64_t out_rs,
+                               int in_dtype, int out_dtype, int act, const float* scale_x, const float* scale_gate,
+                               const float* scale_up, int scale_mode, float* saved_p, float* saved_a, int device,
+                               void* stream);
+
+/* Gradients of hb200_gated_gemm with 16-bit operands, from dh [M,F] and what the forward call saved:
+ *   dG = dh * saved_p, dU = dh * saved_a (rounded to dtype: operands of the products that follow),
+ *   dx = dG @ w_gate^T + dU @ w_up^T,  dw_gate = x^T @ dG,  dw_up = x^T @ dU;  fp32 accumulation.
+ *   dx: [M,K] contiguous, or NULL;  dw_gate, dw_up: [K,F] in the weights' layout without gaps, or both NULL.
+ *   workspace: 2 * M * F * 2 bytes, 16-byte aligned, used on `stream` only.
+ * Layouts and limits as for hb200_gated_gemm; M >= 1. */
+HB200_API int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate, const void* w_up,
+                                        const float* saved_p, const float* saved_a, void* dx, void* dw_gate, void* dw_up,
+                                        int64_t M, int64_t F, int64_t K, int64_t dh_rs, int64_t x_rs, int64_t gate_rs,
+                                        int64_t gate_cs, int64_t up_rs, int64_t up_cs, int dtype, void* workspace,
+                                        size_t workspace_bytes, int device, void* stream);
+
 /* Row-wise quantisation to 8 bits: for each row of x [M,N] one scale and N codes,
  *   scale = max(max|x| / Q, FLT_MIN),  code = round_to_nearest_even(x / scale),  Q = 448 (E4M3) or 127 (INT8),
  * in fp32.  The codes and scales are what hb200_fp8_gemm_scaled / hb200_int8_gemm take as x and scale_a with
