@@ -6,6 +6,7 @@ examples stop at one product with an epilogue (examples/matmul.py:26-56).
 """
 from __future__ import annotations
 
+import weakref
 from typing import Optional
 
 import torch
@@ -31,91 +32,103 @@ def _check_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
 
 def _rows_ready(t: torch.Tensor, per16: int) -> torch.Tensor:
     """``t`` itself where its rows are what the kernels read (unit column stride, 16-byte aligned), else a copy."""
-    if t.stride(1) == 1 and t.stride(0) % per16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+    rs, cs = t.stride()
+    if cs == 1 and rs % per16 == 0 and rs >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _weights_ready(w_gate: torch.Tensor, w_up: torch.Tensor, per16: int, row_major: bool):
     """Both weights in one layout the kernels read: column-major, or row-major where that is allowed and they are."""
-    if row_major and w_gate.stride(1) == 1 and w_up.stride(1) == 1 and w_gate.stride(0) != 1 and w_up.stride(0) != 1:
+    k = w_gate.shape[0]
+    (g0, g1), (u0, u1) = w_gate.stride(), w_up.stride()
+    if g0 == u0 == 1 and g1 >= k and u1 >= k and (g1 | u1) % per16 == 0 and (w_gate.data_ptr() | w_up.data_ptr()) % 16 == 0:
+        return w_gate, w_up
+    if row_major and g1 == u1 == 1 and g0 != 1 and u0 != 1:
         return _rows_ready(w_gate, per16), _rows_ready(w_up, per16)
     return _rows_ready(w_gate.t(), per16).t(), _rows_ready(w_up.t(), per16).t()
 
 
-def _launch(x, w_gate, w_up, out, act: int, scales=(None, None, None), mode: int = _lib.SCALE_NONE, saved=(None, None), what: str = "gated_gemm"):
-    dev = _require_cuda(x, w_gate, w_up, out)
-    ptr = [t.data_ptr() if t is not None else None for t in (*scales, *saved)]
+def _launch(x, w_gate, w_up, out, act: int, dev: int, what: str, scales=(None, None, None), mode: int = _lib.SCALE_NONE, saved=(None, None)):
+    m, k = x.shape
     code = _lib.load().hb200_gated_gemm(
-        x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), x.shape[0], out.shape[1], x.shape[1],
-        x.stride(0), w_gate.stride(0), w_gate.stride(1), w_up.stride(0), w_up.stride(1), out.stride(0),
-        _OUT_DT[x.dtype], _OUT_DT[out.dtype], act, *ptr[:3], mode, *ptr[3:], dev, _stream_ptr(dev),
+        x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), m, out.shape[1], k, x.stride(0),
+        *w_gate.stride(), *w_up.stride(), out.stride(0), _OUT_DT[x.dtype], _OUT_DT[out.dtype], act, *scales, mode, *saved, dev,
+        _stream_ptr(dev),
     )
-    _lib.raise_for(code, what)
+    if code:
+        _lib.raise_for(code, what)
     return out
+
+
+# Backward nodes of eager forward passes on the default stream that are still alive (see _refuse_capture).
+_eager_nodes: "weakref.WeakSet" = weakref.WeakSet()
 
 
 class _GatedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act):
+        dev = x.get_device()
         x = _rows_ready(x, 8)
         w_gate, w_up = _weights_ready(w_gate, w_up, 8, True)
         m, f = x.shape[0], w_gate.shape[1]
-        out = torch.empty((m, f), dtype=x.dtype, device=x.device)
+        out = x.new_empty((m, f))
         # u * act'(g) and act(g) in fp32: the gradients of g and u are then rounded once, as operands of their products
-        p, a = torch.empty((2, m, f), dtype=torch.float32, device=x.device)
-        _launch(x, w_gate, w_up, out, act, saved=(p, a), what="gated_matmul")
-        ctx.save_for_backward(x, w_gate, w_up, p, a)
+        saved = x.new_empty((2, m, f), dtype=torch.float32)
+        p = saved.data_ptr()
+        _launch(x, w_gate, w_up, out, act, dev, "gated_matmul", saved=(p, p + 4 * m * f))
+        ctx.save_for_backward(x, w_gate, w_up, saved)
+        if _stream_ptr(dev) == 0:
+            _eager_nodes.add(ctx)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        x, w_gate, w_up, p, a = ctx.saved_tensors
+        x, w_gate, w_up, saved = ctx.saved_tensors
+        want_x, want_gate, want_up, _ = ctx.needs_input_grad
         m, k = x.shape
         f = w_gate.shape[1]
         dev = _require_cuda(dh, x)
         dh = _rows_ready(dh, 8)
-        dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
-        dw_gate = dw_up = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            if w_gate.stride(0) == 1:
-                dw_gate, dw_up = (torch.empty((f, k), dtype=x.dtype, device=x.device).t() for _ in range(2))
-            else:
-                dw_gate, dw_up = (torch.empty((k, f), dtype=x.dtype, device=x.device) for _ in range(2))
-        workspace = torch.empty((2, m, f), dtype=x.dtype, device=x.device)
-        ptr = [t.data_ptr() if t is not None else None for t in (dx, dw_gate, dw_up)]
+        dx = dw_gate = dw_up = None
+        if want_x:
+            dx = x.new_empty((m, k))
+        if want_gate or want_up:
+            strides = (1, k) if w_gate.stride(0) == 1 else (f, 1)
+            dw_gate, dw_up = x.new_empty_strided((k, f), strides), x.new_empty_strided((k, f), strides)
+        workspace = x.new_empty((2, m, f))
+        p = saved.data_ptr()
         code = _lib.load().hb200_gated_gemm_backward(
-            dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), p.data_ptr(), a.data_ptr(), *ptr, m, f, k,
-            dh.stride(0), x.stride(0), w_gate.stride(0), w_gate.stride(1), w_up.stride(0), w_up.stride(1),
-            _OUT_DT[x.dtype], workspace.data_ptr(), workspace.numel() * workspace.element_size(), dev, _stream_ptr(dev),
+            dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), p, p + 4 * m * f,
+            None if dx is None else dx.data_ptr(), None if dw_gate is None else dw_gate.data_ptr(),
+            None if dw_up is None else dw_up.data_ptr(), m, f, k, dh.stride(0), x.stride(0), *w_gate.stride(), *w_up.stride(),
+            _OUT_DT[x.dtype], workspace.data_ptr(), 4 * m * f, dev, _stream_ptr(dev),
         )
-        _lib.raise_for(code, "gated_matmul backward")
-        return dx, dw_gate if ctx.needs_input_grad[1] else None, dw_up if ctx.needs_input_grad[2] else None, None
+        if code:
+            _lib.raise_for(code, "gated_matmul backward")
+        return dx, dw_gate if want_gate else None, dw_up if want_up else None, None
 
 
-_NODE_STREAM = "helion_b200.stream"  # key in a gradient accumulator's metadata: the stream it was first used on here
+def _refuse_capture(*leaves: torch.Tensor) -> None:
+    """Refuses a capture that living eager graphs over the leaves among ``leaves`` would break.
 
-
-def _accumulators(*leaves: torch.Tensor) -> list:
-    """The gradient accumulators of the leaves among ``leaves``; refuses a capture that their streams would break.
-
-    Autograd ties a leaf's accumulator to the stream it was made on for as long as any graph over that leaf lives.  A
-    backward pass under capture then waits on that stream, which CUDA forbids for the default one: the capture is lost
-    in the middle of the backward pass.  So it is refused here, before anything is recorded.
+    Autograd ties a leaf's gradient accumulator to the stream it was made on for as long as any graph over that leaf
+    lives.  A backward pass under capture then waits on that stream, which CUDA forbids for the default one: the capture
+    would be lost in the middle of the backward pass.  So it is refused here, before anything is recorded.
     """
-    nodes = []
-    for t in leaves:
-        if t.requires_grad and t.grad_fn is None:
-            node = torch.autograd.graph.get_gradient_edge(t).node
-            stream = _stream_ptr(t.device.index)
-            if node.metadata.setdefault(_NODE_STREAM, stream) == 0 and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(
-                    "gated_matmul: an eager graph over the same leaf tensors, made on the default stream, is still alive; "
-                    "a backward pass cannot be captured next to it. Drop its results first, or make it on another stream"
-                )
-            nodes.append(node)
-    return nodes
+    edges = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t.requires_grad and t.grad_fn is None]
+    seen, todo = set(), list(_eager_nodes)
+    while todo:
+        node = todo.pop()
+        if any(node is e for e in edges):
+            raise RuntimeError(
+                "gated_matmul: an eager graph over the same leaf tensors, made on the default stream, is still alive; "
+                "a backward pass cannot be captured next to it. Drop its results first, or make it on another stream"
+            )
+        if node not in seen:
+            seen.add(node)
+            todo += [n for n, _ in node.next_functions if n is not None]
 
 
 def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation: str = "silu") -> torch.Tensor:
@@ -131,13 +144,14 @@ def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"gated_matmul expects three float16 or three bfloat16 tensors, got {x.dtype}, {w_gate.dtype} and {w_up.dtype}")
     act = _check_gated(x, w_gate, w_up, activation, "gated_matmul")
-    _require_cuda(x, w_gate, w_up)
+    dev = _require_cuda(x, w_gate, w_up)
     m, k = x.shape
     f = w_gate.shape[1]
     if m == 0 or f == 0 or k == 0:
         return (x @ w_gate) * (x @ w_up)  # without elements, or zeros: act(0) = 0
     grad = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
-    held = _accumulators(x, w_gate, w_up) if grad else None  # noqa: F841  (alive until the graph holds them)
+    if grad and _eager_nodes and torch.cuda.is_current_stream_capturing():
+        _refuse_capture(x, w_gate, w_up)
     kp, fp = _round_up(k, 8), _round_up(f, 8)
     if kp != k or fp != f:  # odd K or F: the same kernels on zero-padded copies; zero columns give act(0) * 0
         pad = torch.nn.functional.pad
@@ -147,28 +161,29 @@ def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
         return _GatedMatmul.apply(x, w_gate, w_up, act)
     x = _rows_ready(x, 8)
     w_gate, w_up = _weights_ready(w_gate, w_up, 8, True)
-    return _launch(x, w_gate, w_up, torch.empty((m, f), dtype=x.dtype, device=x.device), act, what="gated_matmul")
+    return _launch(x, w_gate, w_up, x.new_empty((m, f)), act, dev, "gated_matmul")
 
 
-def _gated_scales(scale_x, scale_gate, scale_up, m: int, f: int, device):
+def _gated_scales(scale_x, scale_gate, scale_up, m: int, f: int, dev: int):
     """Validate the three scales; returns contiguous fp32 vectors and the C-ABI scale mode."""
     scales = (scale_x, scale_gate, scale_up)
-    if all(s is None for s in scales):
-        return scales, _lib.SCALE_NONE
-    if any(s is None for s in scales):
-        raise ValueError("gated_gemm: pass scale_x, scale_gate and scale_up, or none of them")
+    if scale_x is None or scale_gate is None or scale_up is None:
+        if any(s is not None for s in scales):
+            raise ValueError("gated_gemm: pass scale_x, scale_gate and scale_up, or none of them")
+        return (), _lib.SCALE_NONE
     for name, t in zip(("scale_x", "scale_gate", "scale_up"), scales):
         if t.dtype != torch.float32:
             raise TypeError(f"gated_gemm: {name} must be a float32 tensor")
-        if t.device != device:
+        if t.get_device() != dev:
             raise ValueError(f"gated_gemm: {name} must live on the inputs' device")
+    shapes = scale_x.shape, scale_gate.shape, scale_up.shape
+    if shapes[0] in ((m, 1), (m,)) and shapes[1] in ((1, f), (f,)) and shapes[2] in ((1, f), (f,)):
+        return tuple(s if s.is_contiguous() else s.contiguous() for s in scales), _lib.SCALE_ROWWISE
     if all(s.numel() == 1 for s in scales):
-        return tuple(s.reshape(1) for s in scales), _lib.SCALE_TENSOR
-    if tuple(scale_x.shape) in ((m, 1), (m,)) and all(tuple(s.shape) in ((1, f), (f,)) for s in scales[1:]):
-        return tuple(s.reshape(-1).contiguous() for s in scales), _lib.SCALE_ROWWISE
+        return scales, _lib.SCALE_TENSOR
     raise ValueError(
         "gated_gemm: scales must be one element each, or [M,1]/[M], [1,F]/[F] and [1,F]/[F]; got "
-        f"{tuple(scale_x.shape)}, {tuple(scale_gate.shape)} and {tuple(scale_up.shape)} for M={m}, F={f}"
+        f"{tuple(shapes[0])}, {tuple(shapes[1])} and {tuple(shapes[2])} for M={m}, F={f}"
     )
 
 
@@ -197,12 +212,12 @@ def gated_gemm(
     act = _check_gated(x, w_gate, w_up, activation, "gated_gemm")
     if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TypeError(f"gated_gemm out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
-    _require_cuda(x, w_gate, w_up)
+    dev = _require_cuda(x, w_gate, w_up)
     m, k = x.shape
     f = w_gate.shape[1]
-    scales, mode = _gated_scales(scale_x, scale_gate, scale_up, m, f, x.device)
+    scales, mode = _gated_scales(scale_x, scale_gate, scale_up, m, f, dev)
     if out is None:
-        out = torch.empty((m, f), dtype=out_dtype, device=x.device)
+        out = x.new_empty((m, f), dtype=out_dtype)
     elif out.dtype != out_dtype or tuple(out.shape) != (m, f) or out.stride(1) != 1 or out.device != x.device:
         raise ValueError("gated_gemm: `out` must be a row-major [M, F] tensor of out_dtype on the inputs' device")
     if m == 0 or f == 0:
@@ -219,10 +234,12 @@ def gated_gemm(
             wp[:f, :k].copy_(w.t())
             padded.append(wp.t())
         if mode == _lib.SCALE_ROWWISE:
-            scales = (scales[0], *(torch.nn.functional.pad(s, (0, fp - f)) for s in scales[1:]))
-        res = torch.empty((m, fp), dtype=out_dtype, device=x.device)
-        out.copy_(_launch(xp, *padded, res, act, scales, mode)[:, :f])
+            scales = (scales[0], *(torch.nn.functional.pad(s.reshape(f), (0, fp - f)) for s in scales[1:]))
+        res = x.new_empty((m, fp), dtype=out_dtype)
+        ptrs = tuple(s.data_ptr() for s in scales) or (None, None, None)
+        out.copy_(_launch(xp, *padded, res, act, dev, "gated_gemm", ptrs, mode)[:, :f])
         return out
     x = _rows_ready(x, 16)
     w_gate, w_up = _weights_ready(w_gate, w_up, 16, False)
-    return _launch(x, w_gate, w_up, out, act, scales, mode)
+    ptrs = tuple(s.data_ptr() for s in scales) or (None, None, None)
+    return _launch(x, w_gate, w_up, out, act, dev, "gated_gemm", ptrs, mode)

@@ -28,18 +28,25 @@ _TINY, _HUGE = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def _require_cuda(*tensors: torch.Tensor) -> int:
-    dev = tensors[0].device
-    if dev.type != "cuda":
+    index = tensors[0].get_device()  # -1 on the CPU
+    if not tensors[0].is_cuda:
         raise RuntimeError(
-            f"helion_b200 runs on CUDA (sm_100a) tensors only, got a tensor on {dev}; there is no CPU fallback"
+            f"helion_b200 runs on CUDA (sm_100a) tensors only, got a tensor on {tensors[0].device}; there is no CPU fallback"
         )
     for t in tensors[1:]:
-        if t.device != dev:
-            raise RuntimeError(f"all tensors must be on the same device, got {dev} and {t.device}")
-    return dev.index if dev.index is not None else torch.cuda.current_device()
+        if t.get_device() != index or not t.is_cuda:
+            raise RuntimeError(f"all tensors must be on the same device, got {tensors[0].device} and {t.device}")
+    return index
+
+
+# The current stream's handle without the Stream object around it, where this build of torch offers that (it saves
+# a microsecond of every call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _stream_ptr(device_index: int) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(device_index)
     return torch.cuda.current_stream(device_index).cuda_stream
 
 
@@ -412,37 +419,39 @@ def preprocess_fp8_attention_inputs(
     return q8.reshape(bh, seq, dim), k8.reshape(bh, seq, dim), v8.reshape(bh, seq, dim).permute(0, 2, 1)
 
 
-def _row_view(t: torch.Tensor) -> torch.Tensor:
+def _row_view(t: torch.Tensor, n: int) -> torch.Tensor:
     """``[..., N]`` as rows ``[M, N]`` of unit column stride that do not overlap (a copy only where there is no such view)."""
-    n = t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(math.prod(t.shape[:-1]), n)
-    if t.stride(1) != 1 or t.stride(0) < n:
-        if t.shape[0] > 1 or t.stride(1) != 1:
-            t = t.contiguous()
+    if t.stride(1) != 1 or (t.stride(0) < n and t.shape[0] > 1):
+        t = t.contiguous()
     return t
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _out_rows(out: Optional[torch.Tensor], like: torch.Tensor, shape, dtype: torch.dtype, what: str) -> torch.Tensor:
     """``out`` checked against what the operator would allocate, or that allocation."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     if out.dtype != dtype or out.shape != shape or out.device != like.device or not out.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {list(shape)} tensor of {dtype} on the inputs' device")
     return out
 
 
-def _check_row_input(x: torch.Tensor, out_dtype: torch.dtype, what: str) -> None:
-    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+_ROW_SOURCES = {torch.float16: _lib.DT_FP16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_FP32}
+_ROW_CODES = {torch.float8_e4m3fn: _lib.DT_E4M3, torch.int8: _lib.DT_INT8}
+
+
+def _check_row_input(x: torch.Tensor, out_dtype: torch.dtype, what: str):
+    """The C-ABI type codes of ``x`` and ``out_dtype``."""
+    source = _ROW_SOURCES.get(x.dtype)
+    if source is None:
         raise TypeError(f"{what} expects a float16, bfloat16 or float32 input, got {x.dtype}")
-    if out_dtype not in (torch.float8_e4m3fn, torch.int8):
+    target = _ROW_CODES.get(out_dtype)
+    if target is None:
         raise TypeError(f"{what} out_dtype must be float8_e4m3fn or int8, got {out_dtype}")
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{what} expects rows of at least one value, got shape {tuple(x.shape)}")
+    return source, target
 
 
 def quantize_rows(
@@ -460,20 +469,22 @@ def quantize_rows(
     scale; a NaN makes its row's scale NaN, an infinity makes it infinite.  ``out`` and ``scale_out`` (contiguous)
     take the results of a caller that keeps its buffers.
     """
-    _check_row_input(x, out_dtype, "quantize_rows")
+    source, target = _check_row_input(x, out_dtype, "quantize_rows")
     dev = _require_cuda(x)
-    codes = _out_rows(out, x, x.shape, out_dtype, "quantize_rows: `out`")
-    scales = _out_rows(scale_out, x, (*x.shape[:-1], 1), torch.float32, "quantize_rows: `scale_out`")
-    n = x.shape[-1]
-    rows = _row_view(x)
+    shape = x.shape
+    n = shape[-1]
+    codes = _out_rows(out, x, shape, out_dtype, "quantize_rows: `out`")
+    scales = _out_rows(scale_out, x, (*shape[:-1], 1), torch.float32, "quantize_rows: `scale_out`")
+    rows = _row_view(x, n)
     m = rows.shape[0]
     if m == 0:
         return codes, scales
     code = _lib.load().hb200_quantize_rows(
-        rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, n, _row_stride(rows), n, _OUT_DT[x.dtype],
-        _OUT_DT[out_dtype], dev, _stream_ptr(dev),
+        rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, n, rows.stride(0) if m > 1 else n, n, source, target, dev,
+        _stream_ptr(dev),
     )
-    _lib.raise_for(code, "quantize_rows")
+    if code:
+        _lib.raise_for(code, "quantize_rows")
     return codes, scales
 
 
@@ -494,15 +505,17 @@ def rms_norm_quantize(
     ``[..., 1]`` of ``y`` (see :func:`quantize_rows`) and, when ``residual`` is given, ``s`` in ``x``'s type: the
     residual of the next layer.  The norm takes the fp32 sum before that rounding.  ``x`` and ``residual`` share one
     dtype (fp16, bf16, fp32); ``weight [N]`` has it too or is fp32.  ``residual_out`` may be ``x`` or ``residual``
-    itself (an update in place); ``eps`` is a positive normal fp32 number; ``out``, ``scale_out`` and ``residual_out`` are contiguous.  A row whose sum of
-    squares is not finite in fp32 gets a NaN scale.
+    itself (an update in place); ``eps`` is a positive normal fp32 number; ``out``, ``scale_out`` and ``residual_out``
+    are contiguous.  A row whose sum of squares is not finite in fp32 gets a NaN scale.
     """
-    _check_row_input(x, out_dtype, "rms_norm_quantize")
-    n = x.shape[-1]
+    source, target = _check_row_input(x, out_dtype, "rms_norm_quantize")
+    shape, dtype = x.shape, x.dtype
+    n = shape[-1]
     if weight.dim() != 1 or weight.shape[0] != n:
         raise ValueError(f"rms_norm_quantize: weight must be a vector of N={n} values, got {tuple(weight.shape)}")
-    if weight.dtype != x.dtype and weight.dtype != torch.float32:
-        raise TypeError(f"rms_norm_quantize: weight must be {x.dtype} or float32, got {weight.dtype}")
+    w_type = source if weight.dtype == dtype else _lib.DT_FP32
+    if weight.dtype != dtype and weight.dtype != torch.float32:
+        raise TypeError(f"rms_norm_quantize: weight must be {dtype} or float32, got {weight.dtype}")
     if not _TINY <= eps <= _HUGE:
         raise ValueError(f"rms_norm_quantize: eps must be a positive normal fp32 number, got {eps}")
     if residual is None:
@@ -510,30 +523,32 @@ def rms_norm_quantize(
             raise ValueError("rms_norm_quantize: `residual_out` needs a residual")
         dev = _require_cuda(x, weight)
     else:
-        if residual.dtype != x.dtype:
-            raise TypeError(f"rms_norm_quantize: residual must be {x.dtype} like x, got {residual.dtype}")
-        if residual.shape != x.shape:
-            raise ValueError(f"rms_norm_quantize: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
+        if residual.dtype != dtype:
+            raise TypeError(f"rms_norm_quantize: residual must be {dtype} like x, got {residual.dtype}")
+        if residual.shape != shape:
+            raise ValueError(f"rms_norm_quantize: residual {tuple(residual.shape)} and x {tuple(shape)} differ in shape")
         dev = _require_cuda(x, weight, residual)
-    codes = _out_rows(out, x, x.shape, out_dtype, "rms_norm_quantize: `out`")
-    scales = _out_rows(scale_out, x, (*x.shape[:-1], 1), torch.float32, "rms_norm_quantize: `scale_out`")
-    rows = _row_view(x)
+    codes = _out_rows(out, x, shape, out_dtype, "rms_norm_quantize: `out`")
+    scales = _out_rows(scale_out, x, (*shape[:-1], 1), torch.float32, "rms_norm_quantize: `scale_out`")
+    rows = _row_view(x, n)
     m = rows.shape[0]
     if weight.stride(0) != 1:
         weight = weight.contiguous()
     summed = res_ptr = sum_ptr = None
-    res_rs = 0
+    res_rs = n
     if residual is not None:
-        summed = _out_rows(residual_out, x, x.shape, x.dtype, "rms_norm_quantize: `residual_out`")
-        res = _row_view(residual)
-        res_ptr, sum_ptr, res_rs = res.data_ptr(), summed.data_ptr(), _row_stride(res)
+        summed = _out_rows(residual_out, x, shape, dtype, "rms_norm_quantize: `residual_out`")
+        res = _row_view(residual, n)
+        if m > 1:
+            res_rs = res.stride(0)
+        res_ptr, sum_ptr = res.data_ptr(), summed.data_ptr()
     if m > 0:
         code = _lib.load().hb200_rms_norm_quantize(
             rows.data_ptr(), res_ptr, weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), sum_ptr, m, n,
-            _row_stride(rows), res_rs, n, n, _OUT_DT[x.dtype], _OUT_DT[weight.dtype], _OUT_DT[out_dtype], eps, dev,
-            _stream_ptr(dev),
+            rows.stride(0) if m > 1 else n, res_rs, n, n, source, w_type, target, eps, dev, _stream_ptr(dev),
         )
-        _lib.raise_for(code, "rms_norm_quantize")
+        if code:
+            _lib.raise_for(code, "rms_norm_quantize")
     return (codes, scales) if residual is None else (codes, scales, summed)
 
 
