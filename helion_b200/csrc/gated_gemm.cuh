@@ -6,7 +6,7 @@
 //
 // The structure is that of the 256-row pair kernel of fp8_gemm.cu: two CTAs drive one M = 256 instruction
 // (tcgen05.mma.cta_group::2), each loads its own 128 rows of A and half of the tile's BN columns of B, a TMA warp, an MMA
-// warp and four epilogue warps work on two accumulators in tensor memory.  What is new is where the operands come from:
+// warp and eight epilogue warps work on two accumulators in tensor memory.  What is new is where the operands come from:
 //
 //   GATED: the leader's half of B is BN/2 columns of Wg, the other CTA's half the SAME columns of Wu.  One instruction
 //     then computes g and u of a row side by side in one accumulator, and a thread of the epilogue finds both in its
@@ -30,7 +30,8 @@ enum GatedMode : int { MODE_GATED = 0, MODE_GATED_TRAIN = 1, MODE_SUM = 2, MODE_
 constexpr int GG_BM = 256;      // rows of a pair's tile
 constexpr int GG_BK = 128;      // bytes of K per stage (64 rows of 16-bit values where K is not contiguous)
 constexpr int GG_UMMA_K = 32;   // bytes of K per instruction
-constexpr int GG_THREADS = 192;
+constexpr int GG_EPI_WARPS = 8;
+constexpr int GG_THREADS = 64 + 32 * GG_EPI_WARPS;
 
 template <int BN, int MODE>
 struct GatedLayout {
@@ -40,11 +41,11 @@ struct GatedLayout {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   // staging of one warp: 4 KB for the output, with two more fp32 blocks of 32 x 32 for P and A
   static constexpr int WARP_EPI_BYTES = TRAIN ? 3 * 4096 : 4096;
-  static constexpr int STAGES = BN == 256 ? (TRAIN ? 5 : 6) : (TRAIN ? 7 : 8);
+  static constexpr int STAGES = BN == 256 ? (TRAIN ? 4 : 6) : (TRAIN ? 5 : 8);
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int NUM_BARS = 2 * STAGES + 5;
   static constexpr int EPI_OFFSET = RING_BYTES;
-  static constexpr int BAR_OFFSET = EPI_OFFSET + 4 * WARP_EPI_BYTES;
+  static constexpr int BAR_OFFSET = EPI_OFFSET + GG_EPI_WARPS * WARP_EPI_BYTES;
   static constexpr int MISC_OFFSET = BAR_OFFSET + NUM_BARS * 8;
   static constexpr int SMEM_BYTES = MISC_OFFSET + 16 + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
@@ -114,7 +115,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
   uint64_t* full = bars;                        // used in the leader only
   uint64_t* empty = bars + STAGES;              // one set per CTA
   uint64_t* acc_full = bars + 2 * STAGES;       // one set per CTA
-  uint64_t* acc_empty = bars + 2 * STAGES + 2;  // used in the leader only (8 arrivals: 4 warps x 2 CTAs)
+  uint64_t* acc_empty = bars + 2 * STAGES + 2;  // used in the leader only (one arrival per epilogue warp of both CTAs)
   uint64_t* drain = bars + 2 * STAGES + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC_OFFSET);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::MISC_OFFSET + 4);
@@ -142,7 +143,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);
+      mbar_init(&acc_empty[a], 2 * GG_EPI_WARPS);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -267,6 +268,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
   } else {
     // ------------------------------- epilogue (both CTAs) -------------------------------------
     const int quarter = warp & 3;  // a warp may only touch TMEM lanes [32*(warp%4), +32)
+    const int half = (warp - 2) >> 2;  // two warps share a quarter's columns
     uint8_t* stage = smem + L::EPI_OFFSET + (warp - 2) * L::WARP_EPI_BYTES;
     uint32_t chunk_count = 0;
     uint32_t tile_iter = 0;
@@ -282,7 +284,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
       const int row0 = tc.m_blk * GG_BM + static_cast<int>(rank) * 128 + quarter * 32;
       const uint32_t t_row = tmem_base + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < TILE_N; c += 32, ++chunk_count) {
+      for (int c = half * (TILE_N / 2); c < (half + 1) * (TILE_N / 2); c += 32, ++chunk_count) {
         const int col = tc.n_blk * TILE_N + c;
         const bool inside = row0 < p.M && col < p.N;
         uint32_t r[32];
