@@ -63,7 +63,7 @@ def eight_bit(g, rows, cols, dtype):
     return (torch.randn(rows, cols, generator=g, device="cuda") * 60).clamp(-448, 448).to(E4M3)
 
 
-SIZES = [(1, 16, 8), (1, 4096, 264), (8, 2064, 14336), (17, 144, 19000), (33, 512, 1000), (64, 256, 136), (65, 1040, 520), (128, 272, 128), (129, 128, 72), (257, 2048, 1000), (1000, 512, 5000)]
+SIZES = [(1, 16, 8), (1, 4096, 264), (8, 2064, 14336), (17, 144, 19000), (33, 512, 1000), (64, 256, 136), (65, 1040, 520), (128, 2048, 4224), (96, 4112, 4232), (20, 1024, 9480), (128, 272, 128), (129, 128, 72), (257, 2048, 1000), (1000, 512, 5000)]
 
 
 @pytest.mark.parametrize("out_dtype", list(HALF_STEP), ids=["bf16", "fp16", "fp32"])

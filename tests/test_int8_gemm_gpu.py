@@ -38,7 +38,7 @@ def check(out, x, y, sa=None, sb=None):
 
 @pytest.mark.parametrize("out_dtype", list(HALF_STEP), ids=["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 16), (1, 4096, 256), (16, 14336, 144), (17, 1000, 2048), (33, 24, 4096), (64, 19000, 128), (65, 520, 272),
-                                   (128, 128, 128), (129, 136, 144), (300, 1000, 1040), (1024, 2048, 512), (777, 5000, 2064)])
+                                   (128, 4224, 2048), (100, 4232, 2064), (7, 9472, 1024), (3, 72, 14336), (128, 9480, 528), (128, 128, 128), (129, 136, 144), (300, 1000, 1040), (1024, 2048, 512), (777, 5000, 2064)])
 def test_scaled_products(hb, m, n, k, out_dtype):
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
     x, y = codes(g, m, k), codes(g, n, k).t()
