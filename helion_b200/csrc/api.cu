@@ -71,7 +71,11 @@ DeviceCtx* get_device_ctx(int device) {
                                               std::to_string(prop.major) + std::to_string(prop.minor));
     return nullptr;
   }
+  // The first call on a device may come while this thread captures a graph: the allocation is not part of it.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
   e = cudaHostAlloc(reinterpret_cast<void**>(&c.status_host), 64, cudaHostAllocMapped);
+  cudaThreadExchangeStreamCaptureMode(&mode);
   if (e == cudaSuccess) {
     std::memset(c.status_host, 0, 64);
     e = cudaHostGetDevicePointer(reinterpret_cast<void**>(&c.status_dev), c.status_host, 0);
@@ -743,7 +747,7 @@ static int row_quantize_impl(const char* what, const RowQuantCall& c, int device
   DeviceCtx* ctx = get_device_ctx(device);
   if (ctx == nullptr) return ctx_error_code(device);
   HB_DEVICE_GUARD(device);
-  return launch_row_quantize(c, static_cast<cudaStream_t>(stream));
+  return launch_row_quantize(c, ctx, device, static_cast<cudaStream_t>(stream));
 }
 
 int hb200_quantize_rows(const void* x, void* codes, float* scales, int64_t M, int64_t N, int64_t x_rs, int64_t codes_rs,

@@ -46,6 +46,7 @@ enum WaitSite : uint32_t {
   SITE_ATTN_O_FULL = 18,
   SITE_ATTN_ALPHA = 19,
   SITE_ATTN_O_READY = 20,
+  SITE_ROWS_FULL = 30,
   SITE_SELFTEST = 40,
 };
 

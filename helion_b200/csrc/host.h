@@ -232,7 +232,7 @@ struct RowQuantCall {
   int src_dtype, weight_dtype, out_dtype;
   float eps;
 };
-int launch_row_quantize(const RowQuantCall& c, cudaStream_t stream);
+int launch_row_quantize(const RowQuantCall& c, DeviceCtx* ctx, int device, cudaStream_t stream);
 // The two-tile attention kernel (fp8_attention_pair.cu) on tensor maps built for 128-key steps; non-causal only.
 int launch_fp8_attention_pair(const AttnArgs& args, DeviceCtx* ctx, const CUtensorMap& tq, const CUtensorMap& tk,
                               const CUtensorMap& tv, bool v_kmajor, int poly_of8, bool lazy);

@@ -10,9 +10,10 @@
 // squares and the largest magnitude come out of ONE pass and one block reduction, and rstd does not enter the
 // codes at all.  All of this is fp32; the codes and residual_out are the only roundings to fewer bits.
 //
-// Bound by memory: x (and residual) in, residual_out and one byte a value out.  One CTA takes one row; its values
-// stay in registers between the reduction and the codes, so global memory is touched once.  Rows longer than
-// 1024 threads x 4 groups of 8 are read twice instead (the second time from the L2).
+// Bound by memory: x (and residual) in, residual_out and one byte a value out.  A CTA takes a row at a time; its values
+// stay in registers between the reduction and the codes, so global memory is touched once.  Few rows get a CTA each,
+// many rows persistent CTAs fed by bulk copies (row_ring_kernel).  Rows longer than 1024 threads x 4 groups of 8 are read
+// twice instead (the second time from the L2).
 #include <algorithm>
 #include <atomic>
 
@@ -30,10 +31,18 @@ struct RowQuantArgs {
   void* codes;
   float* scales;
   void* residual_out;
-  int64_t N, x_rs, residual_rs, codes_rs, residual_out_rs;
+  int64_t M, N, x_rs, residual_rs, codes_rs, residual_out_rs;
   float inv_n, eps;
-  bool weight_fp32;  // else of x's type
-  bool int8;         // else e4m3
+  bool weight_fp32;     // else of x's type
+  bool weight_vectors;  // the weight is 16-byte aligned
+  bool int8;            // else e4m3
+};
+
+struct RowQuantLaunch {
+  int64_t M;
+  DeviceCtx* ctx;
+  int device;
+  cudaStream_t stream;
 };
 
 // How a row's groups of 8 values are addressed.
@@ -74,14 +83,16 @@ struct Src<HB200_DT_FP32> {
 };
 
 // Eight values from an aligned address.
-template <int SRC_DT>
+template <int SRC_DT, bool READ_ONLY = false>
 __device__ __forceinline__ void load8(const typename Src<SRC_DT>::T* p, float (&v)[8]) {
   if constexpr (SRC_DT == HB200_DT_FP32) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    const float4* q = reinterpret_cast<const float4*>(p);
+    const float4 a = READ_ONLY ? __ldg(q) : q[0], b = READ_ONLY ? __ldg(q + 1) : q[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    const uint4 u = READ_ONLY ? __ldg(q) : *q;
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -104,21 +115,88 @@ __device__ __forceinline__ void store8(typename Src<SRC_DT>::T* p, const float (
 }
 
 // Values [lo, lo + 8) of a row of N; those outside the row read as zero and are not written.
+// [from, to): where the tensor's values lie, relative to the row.  A group that hangs over its row's end, but not over the
+// tensor's, is read whole and masked (its other values are a neighbouring row's): a branch to eight single loads
+// costs the row's first and last warp a round trip to memory per tensor (1237 x 5003 fp16 with residual: 17.1 us, masked
+// 16.0 us).
 template <int SRC_DT, int TIER>
-__device__ __forceinline__ void load_group(const typename Src<SRC_DT>::T* row, int64_t lo, int64_t N, float (&v)[8]) {
-  if (TIER == ROW_ALIGNED || (TIER == ROW_PHASED && lo >= 0 && lo + 8 <= N)) {
+__device__ __forceinline__ void load_group(const typename Src<SRC_DT>::T* row, int64_t lo, int64_t N, int64_t from, int64_t to,
+                                           float (&v)[8]) {
+  if (TIER == ROW_ALIGNED || (TIER == ROW_PHASED && lo >= from && lo + 8 <= to)) {
     load8<SRC_DT>(row + lo, v);
+    if constexpr (TIER == ROW_PHASED) {
+      if (lo < 0 || lo + 8 > N) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (lo + i >= 0 && lo + i < N) ? v[i] : 0.0f;
+      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (lo + i >= 0 && lo + i < N) ? Src<SRC_DT>::get(row + lo + i) : 0.0f;
   }
 }
 
-// Values [lo, lo + 8) of the weight, whose rows of groups need not be aligned with x's.
+// Eight 16-bit values that begin `shift` (1 to 7) values into the 16 of two neighbouring aligned vectors, `aligned` the
+// second; without the first its values are zeros.
+template <int DT>
+__device__ __forceinline__ void load8_shifted(const typename Src<DT>::T* aligned, bool has_first, int shift, float (&v)[8]) {
+  const uint4 b = __ldg(reinterpret_cast<const uint4*>(aligned));
+  const uint4 a = has_first ? __ldg(reinterpret_cast<const uint4*>(aligned) - 1) : make_uint4(0u, 0u, 0u, 0u);
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  // the shift is the row's, the same in every thread of the CTA
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (shift & 2) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (shift & 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Src<DT>::get2(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// Values [lo, lo + 8) of the weight.  With ROW_PHASED rows lo lies `phase` values before a multiple of 8, where a vector
+// of the weight begins: two vectors and a shift instead of eight loads (1237 x 5003 fp16 with residual: 16.0 us, with the
+// eight loads, as an fp32 weight has them, 18.9 us).
 template <int W_DT, int TIER>
-__device__ __forceinline__ void load_weight(const void* weight, int64_t lo, int64_t N, float (&v)[8]) {
+__device__ __forceinline__ void load_weight_as(const void* weight, int64_t lo, int phase, int64_t N, bool vectors, float (&v)[8]) {
   const auto* w = reinterpret_cast<const typename Src<W_DT>::T*>(weight);
-  load_group<W_DT, TIER == ROW_ALIGNED ? ROW_ALIGNED : ROW_SCALAR>(w, lo, N, v);
+  if constexpr (TIER == ROW_PHASED && W_DT != HB200_DT_FP32) {
+    const int64_t up = lo + phase;  // a multiple of 8
+    if (vectors && up + 8 <= N) {
+      if (phase == 0) load8<W_DT, true>(w + lo, v);
+      else load8_shifted<W_DT>(w + up, up > 0, 8 - phase, v);
+      return;
+    }
+  }
+  if constexpr (TIER == ROW_ALIGNED) {
+    load8<W_DT, true>(w + lo, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (lo + i >= 0 && lo + i < N) ? Src<W_DT>::get(w + lo + i) : 0.0f;
+  }
+}
+
+template <int SRC_DT, int TIER>
+__device__ __forceinline__ void load_weight(const RowQuantArgs& a, int64_t lo, int phase, float (&v)[8]) {
+  if (SRC_DT != HB200_DT_FP32 && a.weight_fp32) load_weight_as<HB200_DT_FP32, TIER>(a.weight, lo, phase, a.N, false, v);
+  else load_weight_as<SRC_DT, TIER>(a.weight, lo, phase, a.N, a.weight_vectors, v);
+}
+
+// Bytes [0, size) of global memory, 16-byte aligned and whole 16-byte pieces, to shared memory.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
 
 template <int SRC_DT, int TIER>
@@ -155,10 +233,54 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t lo, int64_t N,
   }
 }
 
+// One row's factor for the codes, and its scale.
+template <int MODE>
+__device__ __forceinline__ float row_factor(const RowQuantArgs& a, float sum, uint32_t top, float& scale) {
+  const float Q = a.int8 ? 127.0f : 448.0f;
+  constexpr float kTiny = 1.17549435e-38f;
+  const float amax = __uint_as_float(top);
+  float rstd = 1.0f;
+  if constexpr (MODE != 0) {
+    // a sum of squares beyond fp32 (or one that holds an infinity or a NaN) makes the row's scale NaN
+    rstd = sum <= 3.402823466e38f ? 1.0f / sqrtf(sum * a.inv_n + a.eps) : __uint_as_float(0x7fc00000u);
+  }
+  scale = amax * rstd / Q;
+  float f = Q / amax;
+  if (amax < kZeroRow || scale < kTiny) {
+    scale = kTiny;
+    f = 0.0f;
+  }
+  return f;
+}
+
+// Eight values of s w (or x) into the row's sum of squares and largest magnitude; t holds s (or x) on entry.
+template <int MODE>
+__device__ __forceinline__ void take_group(float (&t)[8], const float (&w)[8], float& sum, uint32_t& top) {
+  if constexpr (MODE != 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sum = fmaf(t[i], t[i], sum);
+      t[i] *= w[i];
+    }
+  }
+  // magnitudes compared as bit patterns: a NaN is larger than everything and is not lost
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(t[i]) & kF32AbsMask);
+}
+
+template <int MODE>
+__device__ __forceinline__ void warp_reduce(float& sum, uint32_t& top) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if constexpr (MODE != 0) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+}
+
 // VPT groups of 8 values a thread (0: any number, the row is read twice).  MODE 0: quantise; 1: norm first;
 // 2: norm with the residual's addition.
 template <int SRC_DT, int VPT, int MODE, int TIER>
-__global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
+__global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 512 : 1024) row_quantize_kernel(RowQuantArgs a) {
   using T = typename Src<SRC_DT>::T;
   constexpr int HELD = VPT > 0 ? VPT : 1;
   __shared__ float red_sum[32];
@@ -175,51 +297,51 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
   pdl_wait();
   pdl_launch_dependents();
 
-  // s w (or x) of group g; adds to the sum of squares and the largest magnitude, writes the residual sum
-  auto take = [&](int64_t g, float (&t)[8], float& sum, uint32_t& top, bool write_sum) {
-    const int64_t lo = first + g * 8;
-    load_group<SRC_DT, TIER>(x, lo, a.N, t);
+  // x of group g, and the residual
+  auto load = [&](int64_t g, float (&t)[8], float (&rv)[8]) {
+    load_group<SRC_DT, TIER>(x, first + g * 8, a.N, -row * a.x_rs, (a.M - 1 - row) * a.x_rs + a.N, t);
     if constexpr (MODE == 2) {
-      float rv[8];
-      load_group<SRC_DT, TIER>(r, lo, a.N, rv);
+      load_group<SRC_DT, TIER>(r, first + g * 8, a.N, -row * a.residual_rs, (a.M - 1 - row) * a.residual_rs + a.N, rv);
+    }
+  };
+  // s w (or x) of group g; adds to the sum of squares and the largest magnitude, writes the residual sum
+  auto take = [&](int64_t g, float (&t)[8], const float (&rv)[8], float& sum, uint32_t& top, bool write_sum) {
+    const int64_t lo = first + g * 8;
+    float wv[8];
+    if constexpr (MODE != 0) load_weight<SRC_DT, TIER>(a, lo, static_cast<int>(-first), wv);
+    if constexpr (MODE == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] += rv[i];
       if (write_sum) store_group<SRC_DT, TIER>(s_out, lo, a.N, t);
     }
-    if constexpr (MODE != 0) {
-      float wv[8];
-      if (SRC_DT != HB200_DT_FP32 && a.weight_fp32) load_weight<HB200_DT_FP32, TIER>(a.weight, lo, a.N, wv);
-      else load_weight<SRC_DT, TIER>(a.weight, lo, a.N, wv);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum = fmaf(t[i], t[i], sum);
-        t[i] *= wv[i];
-      }
-    }
-    // magnitudes compared as bit patterns: a NaN is larger than everything and is not lost
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(t[i]) & kF32AbsMask);
+    take_group<MODE>(t, wv, sum, top);
   };
 
-  float t[HELD][8];
+  float t[HELD][8], rv[HELD][8];
   float sum = 0.0f;
   uint32_t top = 0;
   if constexpr (VPT > 0) {
+    // all of a thread's loads before its first store: a store may be to x or the residual itself, so the compiler
+    // cannot move a load over one
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int64_t g = threadIdx.x + static_cast<int64_t>(v) * blockDim.x;
-      if (g < groups) take(g, t[v], sum, top, true);
+      if (g < groups) load(g, t[v], rv[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t g = threadIdx.x + static_cast<int64_t>(v) * blockDim.x;
+      if (g < groups) take(g, t[v], rv[v], sum, top, true);
     }
   } else {
-    for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) take(g, t[0], sum, top, false);
+    for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) {
+      load(g, t[0], rv[0]);
+      take(g, t[0], rv[0], sum, top, false);
+    }
   }
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if constexpr (MODE != 0) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  }
+  warp_reduce<MODE>(sum, top);
   if (warps > 1) {
     if (lane == 0) {
       red_sum[warp] = sum;
@@ -228,27 +350,10 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
     __syncthreads();
     sum = lane < warps ? red_sum[lane] : 0.0f;
     top = lane < warps ? red_max[lane] : 0u;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if constexpr (MODE != 0) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
+    warp_reduce<MODE>(sum, top);
   }
-
-  const float Q = a.int8 ? 127.0f : 448.0f;
-  constexpr float kTiny = 1.17549435e-38f;
-  const float amax = __uint_as_float(top);
-  float rstd = 1.0f;
-  if constexpr (MODE != 0) {
-    // a sum of squares beyond fp32 (or one that holds an infinity or a NaN) makes the row's scale NaN
-    rstd = sum <= 3.402823466e38f ? 1.0f / sqrtf(sum * a.inv_n + a.eps) : __uint_as_float(0x7fc00000u);
-  }
-  float scale = amax * rstd / Q;
-  float f = Q / amax;
-  if (amax < kZeroRow || scale < kTiny) {
-    scale = kTiny;
-    f = 0.0f;
-  }
+  float scale;
+  const float f = row_factor<MODE>(a, sum, top, scale);
   if (threadIdx.x == 0) a.scales[row] = scale;
 
   if constexpr (VPT > 0) {
@@ -261,32 +366,193 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
     for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) {
       float s2 = 0.0f;
       uint32_t t2 = 0;
-      take(g, t[0], s2, t2, true);
+      load(g, t[0], rv[0]);
+      take(g, t[0], rv[0], s2, t2, true);
       store_codes<TIER>(codes, first + g * 8, a.N, t[0], f, a.int8);
     }
   }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Many long rows: persistent CTAs whose rows arrive in a ring of shared-memory stages by bulk copies, so that the memory
+// system stays busy while a row waits for its reduction.  (With a CTA a row, loads and reductions take turns, and the
+// registers of an SM's two to four CTAs hold too few rows in flight.)  A stage is one row of x (and one of the residual);
+// values go to registers on arrival, and the reduction's barrier hands the stage back for the row `stages` ahead.
+//
+// Measured, bf16, a CTA a row / ring: 4096 x 14336 quantised 55.1 / 31.9 us (5.5 TB/s), with norm and residual
+// 85.1 / 68.4 us (6.0 TB/s); 8192 x 4096 quantised 27.0 / 21.1 us, with norm and residual 43.6 / 41.7 us (5.6 TB/s).
+// Below 4096 values a row the CTA-a-row form is as fast or faster (4096 x 2048 with norm 11.7 / 14.4 us), and for rows
+// that are not aligned (1237 x 5003 fp16) the ring gained nothing over it.
+// ------------------------------------------------------------------------------------------------
+constexpr int RING_MAX_STAGES = 8;
+constexpr int RING_SMEM_PER_SM = 220 * 1024;
+
+struct RowRing {
+  int64_t M;
+  int stages;
+  int row_bytes;  // of one tensor
+  uint32_t* status;
+};
+
+template <int SRC_DT, int VPT, int MODE>
+__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) row_ring_kernel(RowQuantArgs a, RowRing ring) {
+  using T = typename Src<SRC_DT>::T;
+  constexpr int TENSORS = MODE == 2 ? 2 : 1;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[RING_MAX_STAGES];
+  __shared__ float red_sum[2][32];
+  __shared__ uint32_t red_max[2][32];
+  __shared__ uint32_t abort_word;
+  volatile uint32_t* abort_flag = &abort_word;
+  const WaitCtx wctx{abort_flag, ring.status};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int groups = static_cast<int>(a.N / 8);
+  const int64_t step = gridDim.x;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring.stages; ++s) mbar_init(&full[s], 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_launch_dependents();
+
+  auto request = [&](int64_t row, int s) {
+    uint8_t* dst = smem + s * TENSORS * ring.row_bytes;
+    mbar_arrive_expect_tx(&full[s], TENSORS * ring.row_bytes);
+    bulk_load(dst, reinterpret_cast<const T*>(a.x) + row * a.x_rs, ring.row_bytes, &full[s]);
+    if constexpr (MODE == 2) {
+      bulk_load(dst + ring.row_bytes, reinterpret_cast<const T*>(a.residual) + row * a.residual_rs, ring.row_bytes, &full[s]);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring.stages; ++s) {
+      if (blockIdx.x + s * step < ring.M) request(blockIdx.x + s * step, s);
+    }
+  }
+
+  int s = 0;
+  uint32_t ph = 0, turn = 0;
+  for (int64_t row = blockIdx.x; row < ring.M; row += step) {
+    const T* sx = reinterpret_cast<const T*>(smem + s * TENSORS * ring.row_bytes);
+    const bool ok = mbar_wait(&full[s], ph, wctx, SITE_ROWS_FULL);
+    float t[VPT][8];
+    float sum = 0.0f;
+    uint32_t top = 0;
+    if (ok) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const int g = threadIdx.x + v * blockDim.x;
+        if (g < groups) {
+          load8<SRC_DT>(sx + g * 8, t[v]);
+          if constexpr (MODE == 2) {
+            float rv[8];
+            load8<SRC_DT>(sx + ring.row_bytes / sizeof(T) + g * 8, rv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[v][i] += rv[i];
+            store8<SRC_DT>(reinterpret_cast<T*>(a.residual_out) + row * a.residual_out_rs + g * 8, t[v]);
+          }
+          float wv[8];
+          if constexpr (MODE != 0) load_weight<SRC_DT, ROW_ALIGNED>(a, g * 8, 0, wv);
+          take_group<MODE>(t[v], wv, sum, top);
+        }
+      }
+    }
+    warp_reduce<MODE>(sum, top);
+    if (lane == 0) {
+      red_sum[turn][warp] = sum;
+      red_max[turn][warp] = top;
+    }
+    // every thread has its values of this stage (or a wait ran out: all leave together)
+    if (!__syncthreads_and(ok)) break;
+    if (threadIdx.x == 0 && row + ring.stages * step < ring.M) request(row + ring.stages * step, s);
+    sum = lane < warps ? red_sum[turn][lane] : 0.0f;
+    top = lane < warps ? red_max[turn][lane] : 0u;
+    warp_reduce<MODE>(sum, top);
+    float scale;
+    const float f = row_factor<MODE>(a, sum, top, scale);
+    if (threadIdx.x == 0) a.scales[row] = scale;
+    uint8_t* codes = reinterpret_cast<uint8_t*>(a.codes) + row * a.codes_rs;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int g = threadIdx.x + v * blockDim.x;
+      if (g < groups) store_codes<ROW_ALIGNED>(codes, g * 8, a.N, t[v], f, a.int8);
+    }
+    turn ^= 1u;
+    if (++s == ring.stages) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+  if (*abort_flag && threadIdx.x == 0) {
+    // give copies that are still in flight time to land before shared memory is released
+    for (int i = 0; i < ring.stages; ++i) {
+      mbar_drain(&full[s], ph);
+      if (++s == ring.stages) {
+        s = 0;
+        ph ^= 1u;
+      }
+    }
+  }
+}
+
+template <int SRC_DT, int VPT, int MODE>
+int launch_ring(const RowQuantArgs& a, const RowRing& ring, int ctas_per_sm, const RowQuantLaunch& l) {
+  auto kernel = row_ring_kernel<SRC_DT, VPT, MODE>;
+  static std::atomic<uint64_t> smem_attr_done{0};
+  HB_CUDA_CHECK(set_max_dynamic_smem_once(smem_attr_done, reinterpret_cast<const void*>(kernel), RING_SMEM_PER_SM, l.device));
+  const int64_t grid = std::min<int64_t>(ring.M, static_cast<int64_t>(l.ctx->num_sms) * ctas_per_sm);
+  const int64_t threads = ((a.N / 8 + VPT - 1) / VPT + 31) / 32 * 32;
+  HB_CUDA_CHECK(launch_pdl(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(threads),
+                           static_cast<size_t>(ring.stages) * ring.row_bytes * (MODE == 2 ? 2 : 1), l.stream, a, ring));
+  return HB200_OK;
+}
+
+// The ring kernel where it applies: rows of 4096 to 16384 values, enough of them that its CTAs loop, at least two in
+// shared memory.  Returns 1 where it does not.
+template <int SRC_DT, int MODE>
+int try_ring(const RowQuantArgs& a, const RowQuantLaunch& l) {
+  if (l.M < 4ll * l.ctx->num_sms || a.N < 4096 || a.N > 16384) return 1;
+  RowRing ring;
+  ring.M = l.M;
+  ring.status = l.ctx->status_dev;
+  ring.row_bytes = static_cast<int>(a.N) * static_cast<int>(sizeof(typename Src<SRC_DT>::T));
+  // as many CTAs an SM as have two stages each: 4 of 256 to 512 threads, 2 of up to 512, 1 of up to 1024
+  for (int ctas = a.N <= 8192 ? 4 : 2; ctas >= 1; ctas /= 2) {
+    ring.stages = std::min(RING_MAX_STAGES, (RING_SMEM_PER_SM / ctas - 2048) / (ring.row_bytes * (MODE == 2 ? 2 : 1)));
+    if (ring.stages < 2) continue;
+    if (ctas == 1 && a.N <= 8192) return launch_ring<SRC_DT, 1, MODE>(a, ring, ctas, l);
+    return ctas == 2 && a.N > 8192 ? launch_ring<SRC_DT, 4, MODE>(a, ring, ctas, l) : launch_ring<SRC_DT, 2, MODE>(a, ring, ctas, l);
+  }
+  return 1;
+}
+
 template <int SRC_DT, int VPT, int MODE, int TIER>
-int launch_row(const RowQuantArgs& a, int64_t M, int threads, cudaStream_t stream) {
-  HB_CUDA_CHECK(launch_pdl(row_quantize_kernel<SRC_DT, VPT, MODE, TIER>, static_cast<unsigned>(M),
-                           static_cast<unsigned>(threads), 0, stream, a));
+int launch_row(const RowQuantArgs& a, const RowQuantLaunch& l, int threads) {
+  HB_CUDA_CHECK(launch_pdl(row_quantize_kernel<SRC_DT, VPT, MODE, TIER>, static_cast<unsigned>(l.M),
+                           static_cast<unsigned>(threads), 0, l.stream, a));
   return HB200_OK;
 }
 
 template <int SRC_DT, int MODE, int TIER>
-int launch_row_size(const RowQuantArgs& a, int64_t M, cudaStream_t stream) {
+int launch_row_size(const RowQuantArgs& a, const RowQuantLaunch& l) {
   const int64_t groups = (a.N + (TIER == ROW_PHASED ? 7 : 0) + 7) / 8;  // a phase adds a group at most
   const int vpt = groups <= 512 ? 1 : (groups <= 1024 ? 2 : 4);
   const int threads = static_cast<int>(std::min<int64_t>(((groups + vpt - 1) / vpt + 31) / 32 * 32, 1024));
   if constexpr (TIER != ROW_SCALAR) {
+    if constexpr (TIER == ROW_ALIGNED) {
+      const int rc = try_ring<SRC_DT, MODE>(a, l);
+      if (rc <= 0) return rc;
+    }
     if (groups <= 4096) {
-      if (vpt == 1) return launch_row<SRC_DT, 1, MODE, TIER>(a, M, threads, stream);
-      if (vpt == 2) return launch_row<SRC_DT, 2, MODE, TIER>(a, M, threads, stream);
-      return launch_row<SRC_DT, 4, MODE, TIER>(a, M, threads, stream);
+      if (vpt == 1) return launch_row<SRC_DT, 1, MODE, TIER>(a, l, threads);
+      if (vpt == 2) return launch_row<SRC_DT, 2, MODE, TIER>(a, l, threads);
+      return launch_row<SRC_DT, 4, MODE, TIER>(a, l, threads);
     }
   }
-  return launch_row<SRC_DT, 0, MODE, TIER>(a, M, threads, stream);
+  return launch_row<SRC_DT, 0, MODE, TIER>(a, l, threads);
 }
 
 // `at` modulo 8 values, or -1 for an address that is not a multiple of the value's size.
@@ -317,27 +583,28 @@ RowTier pick_tier(const RowQuantArgs& a, int mode, int elem, int w_elem) {
 }
 
 template <int SRC_DT, int MODE>
-int launch_row_tier(const RowQuantArgs& a, int64_t M, cudaStream_t stream) {
+int launch_row_tier(const RowQuantArgs& a, const RowQuantLaunch& l) {
   constexpr int elem = sizeof(typename Src<SRC_DT>::T);
   switch (pick_tier(a, MODE, elem, a.weight_fp32 ? 4 : elem)) {
     case ROW_ALIGNED:
-      return launch_row_size<SRC_DT, MODE, ROW_ALIGNED>(a, M, stream);
+      return launch_row_size<SRC_DT, MODE, ROW_ALIGNED>(a, l);
     case ROW_PHASED:
-      return launch_row_size<SRC_DT, MODE, ROW_PHASED>(a, M, stream);
+      return launch_row_size<SRC_DT, MODE, ROW_PHASED>(a, l);
     default:
-      return launch_row_size<SRC_DT, MODE, ROW_SCALAR>(a, M, stream);
+      return launch_row_size<SRC_DT, MODE, ROW_SCALAR>(a, l);
   }
 }
 
 template <int SRC_DT>
-int launch_row_mode(const RowQuantArgs& a, int64_t M, cudaStream_t stream) {
-  if (a.weight == nullptr) return launch_row_tier<SRC_DT, 0>(a, M, stream);
-  return a.residual == nullptr ? launch_row_tier<SRC_DT, 1>(a, M, stream) : launch_row_tier<SRC_DT, 2>(a, M, stream);
+int launch_row_mode(const RowQuantArgs& a, const RowQuantLaunch& l) {
+  if (a.weight == nullptr) return launch_row_tier<SRC_DT, 0>(a, l);
+  return a.residual == nullptr ? launch_row_tier<SRC_DT, 1>(a, l) : launch_row_tier<SRC_DT, 2>(a, l);
 }
 
 }  // namespace
 
-int launch_row_quantize(const RowQuantCall& c, cudaStream_t stream) {
+int launch_row_quantize(const RowQuantCall& c, DeviceCtx* ctx, int device, cudaStream_t stream) {
+  const RowQuantLaunch l{c.M, ctx, device, stream};
   RowQuantArgs a;
   a.x = c.x;
   a.residual = c.residual;
@@ -345,6 +612,7 @@ int launch_row_quantize(const RowQuantCall& c, cudaStream_t stream) {
   a.codes = c.codes;
   a.scales = c.scales;
   a.residual_out = c.residual_out;
+  a.M = c.M;
   a.N = c.N;
   a.x_rs = c.x_rs;
   a.residual_rs = c.residual_rs;
@@ -353,14 +621,15 @@ int launch_row_quantize(const RowQuantCall& c, cudaStream_t stream) {
   a.inv_n = 1.0f / static_cast<float>(c.N);
   a.eps = c.eps;
   a.weight_fp32 = c.weight_dtype == HB200_DT_FP32;
+  a.weight_vectors = reinterpret_cast<uintptr_t>(c.weight) % 16 == 0;
   a.int8 = c.out_dtype == HB200_DT_INT8;
   switch (c.src_dtype) {
     case HB200_DT_FP16:
-      return launch_row_mode<HB200_DT_FP16>(a, c.M, stream);
+      return launch_row_mode<HB200_DT_FP16>(a, l);
     case HB200_DT_BF16:
-      return launch_row_mode<HB200_DT_BF16>(a, c.M, stream);
+      return launch_row_mode<HB200_DT_BF16>(a, l);
     default:
-      return launch_row_mode<HB200_DT_FP32>(a, c.M, stream);
+      return launch_row_mode<HB200_DT_FP32>(a, l);
   }
 }
 

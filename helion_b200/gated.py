@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _OUT_DT, _require_cuda, _round_up, _stream_ptr
+from .ops import _OUT_DT, _empty_matrix, _require_cuda, _round_up, _stream_ptr
 
 _ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
 
@@ -72,9 +72,9 @@ class _GatedMatmul(torch.autograd.Function):
         x = _rows_ready(x, 8)
         w_gate, w_up = _weights_ready(w_gate, w_up, 8, True)
         m, f = x.shape[0], w_gate.shape[1]
-        out = x.new_empty((m, f))
+        out = _empty_matrix(x, m, f, x.dtype)
         # u * act'(g) and act(g) in fp32: the gradients of g and u are then rounded once, as operands of their products
-        saved = x.new_empty((2, m, f), dtype=torch.float32)
+        saved = _empty_matrix(x, 2 * m, f, torch.float32)
         p = saved.data_ptr()
         _launch(x, w_gate, w_up, out, act, dev, "gated_matmul", saved=(p, p + 4 * m * f))
         ctx.save_for_backward(x, w_gate, w_up, saved)
@@ -93,11 +93,11 @@ class _GatedMatmul(torch.autograd.Function):
         dh = _rows_ready(dh, 8)
         dx = dw_gate = dw_up = None
         if want_x:
-            dx = x.new_empty((m, k))
+            dx = _empty_matrix(x, m, k, x.dtype)
         if want_gate or want_up:
             strides = (1, k) if w_gate.stride(0) == 1 else (f, 1)
             dw_gate, dw_up = x.new_empty_strided((k, f), strides), x.new_empty_strided((k, f), strides)
-        workspace = x.new_empty((2, m, f))
+        workspace = _empty_matrix(x, 2 * m, f, x.dtype)
         p = saved.data_ptr()
         code = _lib.load().hb200_gated_gemm_backward(
             dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), p, p + 4 * m * f,
@@ -161,7 +161,7 @@ def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
         return _GatedMatmul.apply(x, w_gate, w_up, act)
     x = _rows_ready(x, 8)
     w_gate, w_up = _weights_ready(w_gate, w_up, 8, True)
-    return _launch(x, w_gate, w_up, x.new_empty((m, f)), act, dev, "gated_matmul")
+    return _launch(x, w_gate, w_up, _empty_matrix(x, m, f, x.dtype), act, dev, "gated_matmul")
 
 
 def _gated_scales(scale_x, scale_gate, scale_up, m: int, f: int, dev: int):
@@ -217,7 +217,7 @@ def gated_gemm(
     f = w_gate.shape[1]
     scales, mode = _gated_scales(scale_x, scale_gate, scale_up, m, f, dev)
     if out is None:
-        out = x.new_empty((m, f), dtype=out_dtype)
+        out = _empty_matrix(x, m, f, out_dtype)
     elif out.dtype != out_dtype or tuple(out.shape) != (m, f) or out.stride(1) != 1 or out.device != x.device:
         raise ValueError("gated_gemm: `out` must be a row-major [M, F] tensor of out_dtype on the inputs' device")
     if m == 0 or f == 0:

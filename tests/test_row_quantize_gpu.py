@@ -9,6 +9,10 @@ code is an 8-bit neighbour of the exact code only where the quotient lies that c
 half a step + 2**-18 of y / scale."""
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -50,7 +54,8 @@ def norm64(x, weight, residual, eps):
 
 @pytest.mark.parametrize("out_dtype", [E4M3, torch.int8], ids=["e4m3", "int8"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("m,n", [(1, 1), (3, 7), (1, 8), (5, 64), (2, 4096), (3, 4099), (33, 5003), (2, 8200), (2, 14336), (2, 32768), (2, 32761), (3, 40000), (2, 50001)])
+@pytest.mark.parametrize("m,n", [(1, 1), (3, 7), (1, 8), (5, 64), (2, 4096), (3, 4099), (33, 5003), (2, 8200), (2, 14336), (2, 32768), (2, 32761), (3, 40000), (2, 50001),
+                                 (592, 1024), (1700, 1031), (900, 4096), (601, 5003), (777, 9000), (650, 14336), (593, 16377), (600, 16384)])
 def test_quantize_rows(hb, m, n, dtype, out_dtype):
     g = torch.Generator(device="cuda").manual_seed(m * 100003 + n)
     x = (torch.randn(m, n, generator=g, device="cuda") * 3.0).to(dtype)
@@ -64,7 +69,7 @@ def test_quantize_rows(hb, m, n, dtype, out_dtype):
 @pytest.mark.parametrize("with_residual", [True, False], ids=["residual", "plain"])
 @pytest.mark.parametrize("out_dtype", [E4M3, torch.int8], ids=["e4m3", "int8"])
 @pytest.mark.parametrize("dtype,w_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16), (torch.float32, torch.float32)])
-@pytest.mark.parametrize("m,n", [(1, 1), (2, 9), (1, 4096), (7, 5003), (2, 14336), (2, 24576), (2, 40001)])
+@pytest.mark.parametrize("m,n", [(1, 1), (2, 9), (1, 4096), (7, 5003), (2, 14336), (2, 24576), (2, 40001), (1190, 1031), (900, 4096), (601, 5003), (650, 14336), (593, 16377), (600, 16384)])
 def test_rms_norm_quantize(hb, m, n, dtype, w_dtype, out_dtype, with_residual):
     g = torch.Generator(device="cuda").manual_seed(m * 100003 + n + 1)
     x = torch.randn(m, n, generator=g, device="cuda").to(dtype)
@@ -101,11 +106,11 @@ def test_leading_dimensions_and_given_buffers(hb):
             assert torch.equal(a.reshape(-1).view(torch.uint8), b.reshape(-1).view(torch.uint8))
 
 
-@pytest.mark.parametrize("n", [40003, 520, 77])
-def test_in_place_on_rows_of_every_kind(hb, n):
-    """Rows read twice (n > 32768), whole and odd: the sum overwrites an input that is still being read."""
+@pytest.mark.parametrize("m,n", [(3, 40003), (3, 520), (3, 77), (1500, 1031), (1500, 4096)])
+def test_in_place_on_rows_of_every_kind(hb, m, n):
+    """Rows read twice (n > 32768), whole and odd, few and many: the sum overwrites an input that is still being read."""
     g = torch.Generator(device="cuda").manual_seed(n)
-    x, r = (torch.randn(3, n, generator=g, device="cuda").half() for _ in range(2))
+    x, r = (torch.randn(m, n, generator=g, device="cuda").half() for _ in range(2))
     w = torch.rand(n, generator=g, device="cuda").half()
     want = hb.rms_norm_quantize(x, w, residual=r)
     got = hb.rms_norm_quantize(x, w, residual=r, residual_out=r)
@@ -128,6 +133,14 @@ def test_strided_and_offset_rows(hb):
         for a, b in zip(got, want):
             assert torch.equal(a.reshape(-1).view(torch.uint8), b.reshape(-1).view(torch.uint8))
         check_codes(*got[:2], norm64(x, wt, r, 1e-6)[1])
+        check_codes(*hb.quantize_rows(x, out_dtype=torch.int8), x.double())
+    # many rows with strides and offsets
+    big = torch.randn(700, 2100, generator=g, device="cuda").bfloat16()
+    w = torch.rand(2100, generator=g, device="cuda")
+    for x, r, wt in ((big[:, 8:2056], big[:, 0:2048], w[:2048]), (big[:, 3:2052], big[:, 11:2060], w[:2049]), (big[:, 3:2052], big[:, 4:2053], w[:2049])):
+        got = hb.rms_norm_quantize(x, wt, residual=r)
+        check_codes(*got[:2], norm64(x, wt, r, 1e-6)[1])  # the order of a row's sum goes by its layout: not the same bits
+        assert torch.equal(got[2], (x.float() + r.float()).bfloat16())
         check_codes(*hb.quantize_rows(x, out_dtype=torch.int8), x.double())
     # a phased row next to guard values: nothing outside the row is written
     store = torch.full((4 * 77 + 32,), 7, dtype=torch.int8, device="cuda")
@@ -161,12 +174,29 @@ def test_rows_of_zeros_tiny_rows_and_rows_that_are_not_finite(hb):
         codes, scales = hb.rms_norm_quantize(small, w, eps=1e-30, out_dtype=out_dtype)
         check_codes(codes, scales, norm64(small, w, None, 1e-30)[1])
     # one infinite or NaN row leaves the others as they were
-    y = torch.randn(3, 256, device="cuda").bfloat16()
-    want = hb.quantize_rows(y)
-    y2 = y.clone()
-    y2[1, 100] = nan
-    got = hb.quantize_rows(y2)
-    assert torch.equal(got[0][::2].view(torch.uint8), want[0][::2].view(torch.uint8)) and torch.equal(got[1][::2], want[1][::2])
+    for m, n in ((3, 256), (1001, 1024)):
+        y = torch.randn(m, n, device="cuda").bfloat16()
+        want = hb.quantize_rows(y)
+        y2 = y.clone()
+        y2[1, 100] = nan
+        got = hb.quantize_rows(y2)
+        assert got[1][1].isnan().all()
+        rest = [i for i in range(m) if i != 1]
+        assert torch.equal(got[0].view(torch.uint8)[rest], want[0].view(torch.uint8)[rest]) and torch.equal(got[1][rest], want[1][rest])
+
+
+def test_the_first_call_of_a_process_may_be_captured(hb):
+    code = """
+import torch, helion_b200 as hb
+x = torch.randn(2, 64, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    codes, scales = hb.quantize_rows(x)
+graph.replay()
+want = hb.quantize_rows(x)
+assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=Path(__file__).resolve().parent.parent, timeout=300)
 
 
 def test_empty_inputs(hb):
