@@ -91,6 +91,7 @@ SIGNATURES = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int,
          _vp, ctypes.c_size_t, ctypes.c_int, _vp],
     ),
+    "hb200_gated_gemm_backward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
     "hb200_quantize_rows": (
         ctypes.c_int,
         [_vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp],

@@ -653,6 +653,14 @@ int hb200_gated_gemm(const void* x, const void* w_gate, const void* w_up, void* 
   return launch_gated(a, ctx);
 }
 
+// Bytes of dG and dU (a multiple of 16: F is one of 8).
+static size_t gated_products_bytes(int64_t M, int64_t F) { return 4 * static_cast<size_t>(M) * static_cast<size_t>(F); }
+
+size_t hb200_gated_gemm_backward_workspace_bytes(int64_t M, int64_t F, int64_t K) {
+  if (M < 1 || F < 1 || K < 1) return 0;
+  return gated_products_bytes(M, F) + gated_grad_partial_bytes(M, F, K, query_num_sms());
+}
+
 int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const float* saved_p,
                               const float* saved_a, void* dx, void* dw_gate, void* dw_up, int64_t M, int64_t F, int64_t K,
                               int64_t dh_rs, int64_t x_rs, int64_t gate_rs, int64_t gate_cs, int64_t up_rs, int64_t up_cs,
@@ -681,10 +689,16 @@ int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate,
   // 4*M*F bytes against the workspace, by division: the product of the sizes cannot wrap that way
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
       static_cast<uint64_t>(M) > workspace_bytes / (4u * static_cast<uint64_t>(F))) {
-    return set_error(HB200_ERR_WORKSPACE, "gated_gemm_backward: needs a 16-byte aligned workspace of 2*M*F 16-bit values");
+    return set_error(HB200_ERR_WORKSPACE, "gated_gemm_backward: needs a 16-byte aligned workspace of "
+                                          "hb200_gated_gemm_backward_workspace_bytes(M, F, K)");
   }
   DeviceCtx* ctx = get_device_ctx(device);
   if (ctx == nullptr) return ctx_error_code(device);
+  const size_t partials_at = gated_products_bytes(M, F);
+  if (dx != nullptr && workspace_bytes < partials_at + gated_grad_partial_bytes(M, F, K, ctx->num_sms)) {
+    return set_error(HB200_ERR_WORKSPACE, "gated_gemm_backward: needs a 16-byte aligned workspace of "
+                                          "hb200_gated_gemm_backward_workspace_bytes(M, F, K)");
+  }
   GatedGradArgs a;
   a.dh = dh;
   a.x = x;
@@ -696,6 +710,7 @@ int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate,
   a.dw[0] = dw_gate;
   a.dw[1] = dw_up;
   a.dgu = workspace;
+  a.partials = static_cast<char*>(workspace) + partials_at;
   a.M = M;
   a.F = F;
   a.K = K;

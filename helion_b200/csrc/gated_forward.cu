@@ -33,6 +33,7 @@ int launch_forward(const GatedArgs& a, DeviceCtx* ctx) {
   p.M = static_cast<int>(a.M);
   p.N = static_cast<int>(a.F);
   p.k_blocks = static_cast<int>((a.K * ES + GG_BK - 1) / GG_BK);
+  p.splits = 1;
   p.group_m = 8;
   p.act = a.act;
   p.status = ctx->status_dev;

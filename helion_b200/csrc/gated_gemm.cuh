@@ -12,7 +12,8 @@
 //     then computes g and u of a row side by side in one accumulator, and a thread of the epilogue finds both in its
 //     own tensor-memory lane: the gate costs no exchange, x is read once for both products, and g and u never leave
 //     the SM.  The tensor pipe does exactly the work of one GEMM of 2F columns.
-//   SUM: the K loop runs over the blocks of the first product and on over those of the second.
+//   SUM: the K loop runs over the blocks of the first product and on over those of the second.  With few tiles the loop
+//     is cut into `splits` units of work (SUM_SPLIT), whose fp32 partial sums a second kernel adds in order.
 //   TWIN: the tile index runs over both products' tiles.
 //   A_MN: A is stored with its rows (M) contiguous, as x and dG are in the weights' gradients; both operands may be.
 #pragma once
@@ -25,7 +26,7 @@
 
 namespace hb {
 
-enum GatedMode : int { MODE_GATED = 0, MODE_GATED_TRAIN = 1, MODE_SUM = 2, MODE_TWIN = 3 };
+enum GatedMode : int { MODE_GATED = 0, MODE_GATED_TRAIN = 1, MODE_SUM = 2, MODE_TWIN = 3, MODE_SUM_SPLIT = 4 };
 
 constexpr int GG_BM = 256;      // rows of a pair's tile
 constexpr int GG_BK = 128;      // bytes of K per stage (64 rows of 16-bit values where K is not contiguous)
@@ -60,6 +61,7 @@ struct GatedMaps {
 struct GatedParams {
   int M, N;        // rows and columns of out (of each out for TWIN); N counts gated columns for GATED
   int k_blocks;    // stages per product
+  int splits;      // SUM_SPLIT: units the K loop is cut into
   int group_m;
   int act;
   uint32_t* status;
@@ -129,8 +131,11 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
   const int m_tiles = (p.M + GG_BM - 1) / GG_BM;
   const int n_tiles = (p.N + TILE_N - 1) / TILE_N;
   const int one = m_tiles * n_tiles;                  // tiles of one product
-  const int num_tiles = MODE == MODE_TWIN ? 2 * one : one;
-  const int k_total = MODE == MODE_SUM ? 2 * p.k_blocks : p.k_blocks;
+  constexpr bool SUM = MODE == MODE_SUM || MODE == MODE_SUM_SPLIT;
+  constexpr bool LAYERS = MODE == MODE_TWIN || MODE == MODE_SUM_SPLIT;  // one tile of out belongs to several units
+  const int num_tiles = MODE == MODE_TWIN ? 2 * one : (MODE == MODE_SUM_SPLIT ? p.splits * one : one);
+  const int k_all = SUM ? 2 * p.k_blocks : p.k_blocks;
+  const int k_unit = MODE == MODE_SUM_SPLIT ? (k_all + p.splits - 1) / p.splits : k_all;
   const WaitCtx wctx{abort_flag, p.status};
 
   if (threadIdx.x == 0) {
@@ -168,19 +173,21 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
       uint32_t it = 0;
       bool ok = true;
       for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
-        const int twin = MODE == MODE_TWIN && tile >= one ? 1 : 0;
-        const TileCoord tc = tile_coord(tile - twin * one, m_tiles, n_tiles, p.group_m);
+        const int layer = LAYERS ? tile / one : 0;
+        const TileCoord tc = tile_coord(tile - layer * one, m_tiles, n_tiles, p.group_m);
+        const int k_begin = MODE == MODE_SUM_SPLIT ? layer * k_unit : 0;
+        const int k_end = min(k_begin + k_unit, k_all);
         const int row0 = tc.m_blk * GG_BM + static_cast<int>(rank) * 128;
         const int col0 = GATED ? tc.n_blk * TILE_N : tc.n_blk * BN + static_cast<int>(rank) * (BN / 2);
-        for (int kt = 0; kt < k_total; ++kt, ++it) {
+        for (int kt = k_begin; kt < k_end; ++kt, ++it) {
           const uint32_t s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1u;
           if (!mbar_wait(&empty[s], ph ^ 1u, wctx, SITE_GEMM_EMPTY)) {
             ok = false;
             break;
           }
-          const int second = MODE == MODE_SUM ? (kt >= p.k_blocks ? 1 : 0) : twin;
-          const int kb = MODE == MODE_SUM ? kt - second * p.k_blocks : kt;
+          const int second = SUM ? (kt >= p.k_blocks ? 1 : 0) : layer;
+          const int kb = SUM ? kt - second * p.k_blocks : kt;
           const CUtensorMap* ma = &maps.a[second];
           const CUtensorMap* mb = &maps.b[GATED ? static_cast<int>(rank) : second];
           uint8_t* a_dst = smem + s * L::STAGE_BYTES;
@@ -229,7 +236,9 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
         }
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kt = 0; kt < k_total; ++kt, ++it) {
+        const int k_begin = MODE == MODE_SUM_SPLIT ? tile / one * k_unit : 0;
+        const int k_end = min(k_begin + k_unit, k_all);
+        for (int kt = k_begin; kt < k_end; ++kt, ++it) {
           const uint32_t s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1u;
           if (!mbar_wait(&full[s], ph, wctx, SITE_GEMM_FULL)) {
@@ -247,7 +256,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
           for (int k = 0; k < GG_BK / GG_UMMA_K; ++k) {
             const uint64_t ad = desc_advance(a_desc, k * (A_MN ? GG_UMMA_K / ES * 128 : GG_UMMA_K));
             const uint64_t bd = desc_advance(b_desc, k * (B_MN ? GG_UMMA_K / ES * 128 : GG_UMMA_K));
-            umma_ss_pair<KIND>(d_tmem, ad, bd, idesc, (kt | k) != 0 ? 1u : 0u);
+            umma_ss_pair<KIND>(d_tmem, ad, bd, idesc, kt != k_begin || k != 0 ? 1u : 0u);
           }
           const uint32_t e_local = smem_u32(&empty[s]);
           umma_commit_pair(e_local);
@@ -273,8 +282,8 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
     uint32_t chunk_count = 0;
     uint32_t tile_iter = 0;
     for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++tile_iter) {
-      const int twin = MODE == MODE_TWIN && tile >= one ? 1 : 0;
-      const TileCoord tc = tile_coord(tile - twin * one, m_tiles, n_tiles, p.group_m);
+      const int layer = LAYERS ? tile / one : 0;
+      const TileCoord tc = tile_coord(tile - layer * one, m_tiles, n_tiles, p.group_m);
       const uint32_t acc = tile_iter & 1u;
       const uint32_t acc_ph = (tile_iter >> 1) & 1u;
       bool ok = mbar_wait(&acc_full[acc], acc_ph, wctx, SITE_GEMM_ACC_FULL);
@@ -312,7 +321,12 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
           }
         } else {
           tmem_wait_ld();
-          StagedStore<OUT_DT>::store(r, stage, chunk_count, lane, &maps.out[twin], col, row0, inside);
+          if constexpr (MODE == MODE_SUM_SPLIT) {
+            constexpr int KEEP = StagedStore<OUT_DT>::NBUF - 1;
+            StagedStore<OUT_DT>::template store<KEEP, true>(r, stage, chunk_count, lane, &maps.out[0], col, row0, inside, nullptr, layer);
+          } else {
+            StagedStore<OUT_DT>::store(r, stage, chunk_count, lane, &maps.out[layer], col, row0, inside);
+          }
         }
       }
       tc_fence_before_sync();
@@ -359,6 +373,14 @@ inline int gated_out_map(CUtensorMap* map, void* base, int64_t m, int64_t n, int
                      fp32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+// The same for `layers` fp32 matrices one after another.
+inline int gated_out_map_layers(CUtensorMap* map, void* base, int64_t m, int64_t n, int layers) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m), static_cast<uint64_t>(layers)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(n) * 4, static_cast<uint64_t>(m) * static_cast<uint64_t>(n) * 4};
+  const uint32_t box[3] = {32, 32, 1};
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 // Whether 128-column tiles finish earlier than 256-column ones: rounds of tiles over the CTA pairs times a tile's
 // length, in which the narrow tile reads 3/4 of the operand bytes for half the products.
 inline bool gated_narrow_tiles(int64_t m, int64_t columns, int products, int num_sms) {
@@ -377,7 +399,7 @@ int launch_gated_pair(const GatedMaps& maps, const GatedParams& p, DeviceCtx* ct
   static std::atomic<uint64_t> smem_attr_done{0};
   HB_CUDA_CHECK(set_max_dynamic_smem_once(smem_attr_done, reinterpret_cast<const void*>(kernel), L::SMEM_BYTES, device));
   const int64_t tiles = ((p.M + static_cast<int64_t>(GG_BM) - 1) / GG_BM) * ((p.N + static_cast<int64_t>(TILE_N) - 1) / TILE_N) *
-                        (MODE == MODE_TWIN ? 2 : 1);
+                        (MODE == MODE_TWIN ? 2 : (MODE == MODE_SUM_SPLIT ? p.splits : 1));
   const int pairs = static_cast<int>(tiles < ctx->num_sms / 2 ? tiles : ctx->num_sms / 2);
   HB_CUDA_CHECK(launch_pdl(kernel, static_cast<unsigned>(2 * pairs), GG_THREADS, L::SMEM_BYTES, stream, maps, p));
   return HB200_OK;

@@ -38,10 +38,11 @@ struct StagedStore {
   static constexpr int STG_BYTES = 32 * ROW_BYTES;
   static constexpr int NBUF = OUT32 ? 1 : 2;  // 4 KB per warp either way
 
-  template <int KEEP = NBUF - 1>
+  // `layer` (with SLICED maps): which of the matrices of a three-dimensional output map the block goes to.
+  template <int KEEP = NBUF - 1, bool SLICED = false>
   __device__ static __forceinline__ void store(const uint32_t (&r)[32], uint8_t* stage, uint32_t chunk_count, int lane,
                                                const CUtensorMap* tmap_out, int col, int row0, bool inside,
-                                               unsigned long long* trace = nullptr) {
+                                               unsigned long long* trace = nullptr, int layer = 0) {
     uint8_t* buf = stage + (chunk_count % NBUF) * STG_BYTES;
     if (lane == 0) tma_store_wait_read<KEEP>();
     __syncwarp();
@@ -75,7 +76,10 @@ struct StagedStore {
     __syncwarp();
     if (lane == 0) {
       // blocks that lie wholly outside the matrix are not stored at all (partial ones are clipped)
-      if (inside) tma_store_2d(tmap_out, buf, col, row0);
+      if (inside) {
+        if constexpr (SLICED) tma_store_3d(tmap_out, buf, col, row0, layer);
+        else tma_store_2d(tmap_out, buf, col, row0);
+      }
       tma_store_commit();
     }
   }

@@ -97,13 +97,15 @@ class _GatedMatmul(torch.autograd.Function):
         if want_gate or want_up:
             strides = (1, k) if w_gate.stride(0) == 1 else (f, 1)
             dw_gate, dw_up = x.new_empty_strided((k, f), strides), x.new_empty_strided((k, f), strides)
-        workspace = _empty_matrix(x, 2 * m, f, x.dtype)
+        lib = _lib.load()
+        bytes_ = lib.hb200_gated_gemm_backward_workspace_bytes(m, f, k)
+        workspace = _empty_matrix(x, 1, bytes_, torch.uint8)
         p = saved.data_ptr()
-        code = _lib.load().hb200_gated_gemm_backward(
+        code = lib.hb200_gated_gemm_backward(
             dh.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), p, p + 4 * m * f,
             None if dx is None else dx.data_ptr(), None if dw_gate is None else dw_gate.data_ptr(),
             None if dw_up is None else dw_up.data_ptr(), m, f, k, dh.stride(0), x.stride(0), *w_gate.stride(), *w_up.stride(),
-            _OUT_DT[x.dtype], workspace.data_ptr(), 4 * m * f, dev, _stream_ptr(dev),
+            _OUT_DT[x.dtype], workspace.data_ptr(), bytes_, dev, _stream_ptr(dev),
         )
         if code:
             _lib.raise_for(code, "gated_matmul backward")

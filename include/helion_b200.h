@@ -236,13 +236,17 @@ HB200_API int hb200_gated_gemm(const void* x, const void* w_gate, const void* w_
  *   dG = dh * saved_p, dU = dh * saved_a (rounded to dtype: operands of the products that follow),
  *   dx = dG @ w_gate^T + dU @ w_up^T,  dw_gate = x^T @ dG,  dw_up = x^T @ dU;  fp32 accumulation.
  *   dx: [M,K] contiguous, or NULL;  dw_gate, dw_up: [K,F] in the weights' layout without gaps, or both NULL.
- *   workspace: 2 * M * F * 2 bytes, 16-byte aligned, used on `stream` only.
+ *   workspace: hb200_gated_gemm_backward_workspace_bytes(M, F, K) of device memory, 16-byte aligned, used on `stream` only.
  * Layouts and limits as for hb200_gated_gemm; M >= 1. */
 HB200_API int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate, const void* w_up,
                                         const float* saved_p, const float* saved_a, void* dx, void* dw_gate, void* dw_up,
                                         int64_t M, int64_t F, int64_t K, int64_t dh_rs, int64_t x_rs, int64_t gate_rs,
                                         int64_t gate_cs, int64_t up_rs, int64_t up_cs, int dtype, void* workspace,
                                         size_t workspace_bytes, int device, void* stream);
+
+/* Bytes of workspace hb200_gated_gemm_backward needs on the current device: dG and dU, and partial sums of dx where few
+ * rows and columns of it leave it to be split along F. */
+HB200_API size_t hb200_gated_gemm_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 
 /* Row-wise quantisation to 8 bits: for each row of x [M,N] one scale and N codes,
  *   scale = max(max|x| / Q, FLT_MIN),  code = round_to_nearest_even(x / scale),  Q = 448 (E4M3) or 127 (INT8),
