@@ -90,11 +90,11 @@ GatedParams grad_params(int64_t m, int64_t n, int64_t k_elems, DeviceCtx* ctx) {
 }
 
 // dx [M,K] = dG Wg^T + dU Wu^T: contracted over F, along which a row-major w is contiguous and a column-major one is not.
-template <int KIND, int DT, bool B_MN, int BN>
+template <int KIND, int DT, bool B_MN, int BN, int MODE = MODE_SUM>
 int launch_grad_input(const GatedGradArgs& a, DeviceCtx* ctx, const void* const dgu[2]) {
   GatedMaps maps;
   for (int i = 0; i < 2; ++i) {
-    int rc = gated_operand_map(&maps.a[i], dgu[i], false, a.F, a.M, a.F, 2, 128);
+    int rc = gated_operand_map(&maps.a[i], dgu[i], false, a.F, a.M, a.F, 2, MODE == MODE_SUM_TALL ? 256 : 128);
     if (rc != HB200_OK) return rc;
     rc = gated_operand_map(&maps.b[i], a.w[i], B_MN, a.F, a.K, a.ldb[i], 2, BN / 2);
     if (rc != HB200_OK) return rc;
@@ -102,7 +102,7 @@ int launch_grad_input(const GatedGradArgs& a, DeviceCtx* ctx, const void* const 
   const int rc = gated_out_map(&maps.out[0], a.dx, a.M, a.K, a.K, false);
   if (rc != HB200_OK) return rc;
   maps.out[1] = maps.out[2] = maps.out[0];
-  return launch_gated_pair<KIND, false, B_MN, BN, MODE_SUM, DT>(maps, grad_params(a.M, a.K, a.F, ctx), ctx, a.device, a.stream);
+  return launch_gated_pair<KIND, false, B_MN, BN, MODE, DT>(maps, grad_params(a.M, a.K, a.F, ctx), ctx, a.device, a.stream);
 }
 
 // Units the K loop of dx is cut into: where its tiles leave half of the CTA pairs idle, as many as occupy them, with at
@@ -111,6 +111,14 @@ int grad_input_splits(int64_t M, int64_t F, int64_t K, int num_sms) {
   const int64_t tiles = ((M + GG_BM - 1) / GG_BM) * ((K + 255) / 256);
   const int64_t fit = std::min<int64_t>(num_sms / 2 / tiles, 2 * ((F + 63) / 64) / 8);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fit, 8)));
+}
+
+// Tall tiles for dx where they need no more than half the rounds over the CTA pairs that 256-row tiles need.
+bool grad_input_tall(int64_t M, int64_t K, int num_sms) {
+  const int64_t pairs = num_sms / 2, columns = (K + 255) / 256;
+  const int64_t tall = ((M + 511) / 512 * columns + pairs - 1) / pairs;
+  const int64_t flat = ((M + 255) / 256 * columns + pairs - 1) / pairs;
+  return 2 * tall <= flat;
 }
 
 template <int KIND, int DT, bool B_MN>
@@ -176,6 +184,9 @@ int launch_grad(const GatedGradArgs& a, DeviceCtx* ctx) {
     if (splits > 1) {
       rc = a.w_colmajor ? launch_grad_input_split<KIND, DT, true>(a, ctx, dgu, splits)
                         : launch_grad_input_split<KIND, DT, false>(a, ctx, dgu, splits);
+    } else if (grad_input_tall(a.M, a.K, ctx->num_sms)) {
+      rc = a.w_colmajor ? launch_grad_input<KIND, DT, true, 256, MODE_SUM_TALL>(a, ctx, dgu)
+                        : launch_grad_input<KIND, DT, false, 256, MODE_SUM_TALL>(a, ctx, dgu);
     } else if (a.w_colmajor) {
       rc = narrow ? launch_grad_input<KIND, DT, true, 128>(a, ctx, dgu) : launch_grad_input<KIND, DT, true, 256>(a, ctx, dgu);
     } else {

@@ -14,6 +14,8 @@
 //     the SM.  The tensor pipe does exactly the work of one GEMM of 2F columns.
 //   SUM: the K loop runs over the blocks of the first product and on over those of the second.  With few tiles the loop
 //     is cut into `splits` units of work (SUM_SPLIT), whose fp32 partial sums a second kernel adds in order.
+//     SUM_TALL has 512 rows a pair (256 a CTA, in two accumulators that fill tensor memory): a quarter less operand
+//     traffic per product, for an epilogue that the next tile's products do not overlap.
 //   TWIN: the tile index runs over both products' tiles.
 //   A_MN: A is stored with its rows (M) contiguous, as x and dG are in the weights' gradients; both operands may be.
 #pragma once
@@ -26,9 +28,9 @@
 
 namespace hb {
 
-enum GatedMode : int { MODE_GATED = 0, MODE_GATED_TRAIN = 1, MODE_SUM = 2, MODE_TWIN = 3, MODE_SUM_SPLIT = 4 };
+enum GatedMode : int { MODE_GATED = 0, MODE_GATED_TRAIN = 1, MODE_SUM = 2, MODE_TWIN = 3, MODE_SUM_SPLIT = 4, MODE_SUM_TALL = 5 };
 
-constexpr int GG_BM = 256;      // rows of a pair's tile
+constexpr int GG_BM = 256;      // rows of a pair's instruction
 constexpr int GG_BK = 128;      // bytes of K per stage (64 rows of 16-bit values where K is not contiguous)
 constexpr int GG_UMMA_K = 32;   // bytes of K per instruction
 constexpr int GG_EPI_WARPS = 8;
@@ -37,12 +39,14 @@ constexpr int GG_THREADS = 64 + 32 * GG_EPI_WARPS;
 template <int BN, int MODE>
 struct GatedLayout {
   static constexpr bool TRAIN = MODE == MODE_GATED_TRAIN;
-  static constexpr int A_BYTES = 128 * GG_BK;
+  static constexpr bool TALL = MODE == MODE_SUM_TALL;
+  static constexpr int A_BYTES = (TALL ? 256 : 128) * GG_BK;
   static constexpr int B_BYTES = BN / 2 * GG_BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  // staging of one warp: 4 KB for the output, with two more fp32 blocks of 32 x 32 for P and A
-  static constexpr int WARP_EPI_BYTES = TRAIN ? 3 * 4096 : 4096;
-  static constexpr int STAGES = BN == 256 ? (TRAIN ? 4 : 6) : (TRAIN ? 5 : 8);
+  // staging of one warp: 4 KB for the output; TRAIN: 2 KB for the output and an fp32 block of 32 x 32 that P and A
+  // take turns in (a second one would cost a stage of operands)
+  static constexpr int WARP_EPI_BYTES = TRAIN ? 2048 + 4096 : 4096;
+  static constexpr int STAGES = TALL ? 4 : (BN == 256 ? (TRAIN ? 5 : 6) : (TRAIN ? 7 : 8));
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
   static constexpr int NUM_BARS = 2 * STAGES + 5;
   static constexpr int EPI_OFFSET = RING_BYTES;
@@ -51,6 +55,7 @@ struct GatedLayout {
   static constexpr int SMEM_BYTES = MISC_OFFSET + 16 + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static_assert(!TALL || BN == 256, "two accumulators of a tall tile fill tensor memory");
 };
 
 struct GatedMaps {
@@ -110,6 +115,9 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
   constexpr int KROWS = GG_BK / ES;  // K rows of a stage whose K is not contiguous
   constexpr bool GATED = MODE == MODE_GATED || MODE == MODE_GATED_TRAIN;
   constexpr int TILE_N = GATED ? BN / 2 : BN;  // columns of out per tile
+  constexpr bool TALL = L::TALL;
+  constexpr int TILE_M = TALL ? 2 * GG_BM : GG_BM;
+  static_assert(!(TALL && A_MN), "the tall tile is built for an A with K contiguous");
   constexpr int HALF_BLOCKS = BN / 2 * ES / 128;  // 128-byte column blocks of this CTA's half of an MN-major B
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -128,10 +136,10 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
   const bool leader = rank == 0;
   const int pair_id = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
-  const int m_tiles = (p.M + GG_BM - 1) / GG_BM;
+  const int m_tiles = (p.M + TILE_M - 1) / TILE_M;
   const int n_tiles = (p.N + TILE_N - 1) / TILE_N;
   const int one = m_tiles * n_tiles;                  // tiles of one product
-  constexpr bool SUM = MODE == MODE_SUM || MODE == MODE_SUM_SPLIT;
+  constexpr bool SUM = MODE == MODE_SUM || MODE == MODE_SUM_SPLIT || TALL;
   constexpr bool LAYERS = MODE == MODE_TWIN || MODE == MODE_SUM_SPLIT;  // one tile of out belongs to several units
   const int num_tiles = MODE == MODE_TWIN ? 2 * one : (MODE == MODE_SUM_SPLIT ? p.splits * one : one);
   const int k_all = SUM ? 2 * p.k_blocks : p.k_blocks;
@@ -148,7 +156,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 2 * GG_EPI_WARPS);
+      mbar_init(&acc_empty[a], TALL ? GG_EPI_WARPS : 2 * GG_EPI_WARPS);  // the warps that drain it, of both CTAs
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -177,7 +185,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
         const TileCoord tc = tile_coord(tile - layer * one, m_tiles, n_tiles, p.group_m);
         const int k_begin = MODE == MODE_SUM_SPLIT ? layer * k_unit : 0;
         const int k_end = min(k_begin + k_unit, k_all);
-        const int row0 = tc.m_blk * GG_BM + static_cast<int>(rank) * 128;
+        const int row0 = tc.m_blk * TILE_M + static_cast<int>(rank) * (TILE_M / 2);
         const int col0 = GATED ? tc.n_blk * TILE_N : tc.n_blk * BN + static_cast<int>(rank) * (BN / 2);
         for (int kt = k_begin; kt < k_end; ++kt, ++it) {
           const uint32_t s = it % STAGES;
@@ -228,8 +236,9 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
       uint32_t tile_iter = 0;
       bool ok = true;
       for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs, ++tile_iter) {
-        const uint32_t acc = tile_iter & 1u;
-        const uint32_t acc_ph = (tile_iter >> 1) & 1u;
+        // tiles take turns with the two accumulators; a tall tile fills both, each handed back on its own
+        const uint32_t acc = TALL ? 0u : tile_iter & 1u;
+        const uint32_t acc_ph = TALL ? tile_iter & 1u : (tile_iter >> 1) & 1u;
         if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, wctx, SITE_GEMM_ACC_EMPTY)) {
           ok = false;
           break;
@@ -250,14 +259,25 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
           const uint32_t b_addr = a_addr + L::A_BYTES;
           // K contiguous: 128-byte rows, 8-row atoms 1024 bytes apart.  M / N contiguous: 128-byte blocks KROWS*128
           // bytes apart, 8 K rows per atom; an instruction consumes UMMA_K/ES rows of K.
-          const uint64_t a_desc = make_smem_desc(a_addr, A_MN ? KROWS * 128 : 16, 1024, SWZ_128B);
           const uint64_t b_desc = make_smem_desc(b_addr, B_MN ? KROWS * 128 : 16, 1024, SWZ_128B);
 #pragma unroll
-          for (int k = 0; k < GG_BK / GG_UMMA_K; ++k) {
-            const uint64_t ad = desc_advance(a_desc, k * (A_MN ? GG_UMMA_K / ES * 128 : GG_UMMA_K));
-            const uint64_t bd = desc_advance(b_desc, k * (B_MN ? GG_UMMA_K / ES * 128 : GG_UMMA_K));
-            umma_ss_pair<KIND>(d_tmem, ad, bd, idesc, kt != k_begin || k != 0 ? 1u : 0u);
+          for (int h = 0; h < (TALL ? 2 : 1); ++h) {
+            if (TALL && h == 1 && kt == k_begin) {
+              if (!mbar_wait(&acc_empty[1], acc_ph ^ 1u, wctx, SITE_GEMM_ACC_EMPTY)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after_sync();
+            }
+            const uint64_t a_desc = make_smem_desc(a_addr + h * (128 * GG_BK), A_MN ? KROWS * 128 : 16, 1024, SWZ_128B);
+#pragma unroll
+            for (int k = 0; k < GG_BK / GG_UMMA_K; ++k) {
+              const uint64_t ad = desc_advance(a_desc, k * (A_MN ? GG_UMMA_K / ES * 128 : GG_UMMA_K));
+              const uint64_t bd = desc_advance(b_desc, k * (B_MN ? GG_UMMA_K / ES * 128 : GG_UMMA_K));
+              umma_ss_pair<KIND>(d_tmem + h * BN, ad, bd, idesc, kt != k_begin || k != 0 ? 1u : 0u);
+            }
           }
+          if (!ok) break;
           const uint32_t e_local = smem_u32(&empty[s]);
           umma_commit_pair(e_local);
           umma_commit_pair(map_to_cta(e_local, 1));
@@ -277,23 +297,24 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
   } else {
     // ------------------------------- epilogue (both CTAs) -------------------------------------
     const int quarter = warp & 3;  // a warp may only touch TMEM lanes [32*(warp%4), +32)
-    const int half = (warp - 2) >> 2;  // two warps share a quarter's columns
+    const int half = (warp - 2) >> 2;  // two warps share a quarter's columns (a tall tile: one for each accumulator)
+    const int c_begin = TALL ? 0 : half * (TILE_N / 2), c_end = TALL ? TILE_N : (half + 1) * (TILE_N / 2);
     uint8_t* stage = smem + L::EPI_OFFSET + (warp - 2) * L::WARP_EPI_BYTES;
     uint32_t chunk_count = 0;
     uint32_t tile_iter = 0;
     for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++tile_iter) {
       const int layer = LAYERS ? tile / one : 0;
       const TileCoord tc = tile_coord(tile - layer * one, m_tiles, n_tiles, p.group_m);
-      const uint32_t acc = tile_iter & 1u;
-      const uint32_t acc_ph = (tile_iter >> 1) & 1u;
-      bool ok = mbar_wait(&acc_full[acc], acc_ph, wctx, SITE_GEMM_ACC_FULL);
+      const uint32_t acc = TALL ? static_cast<uint32_t>(half) : tile_iter & 1u;
+      const uint32_t acc_ph = TALL ? tile_iter & 1u : (tile_iter >> 1) & 1u;
+      bool ok = mbar_wait(&acc_full[TALL ? 0 : acc], acc_ph, wctx, SITE_GEMM_ACC_FULL);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after_sync();
-      const int row0 = tc.m_blk * GG_BM + static_cast<int>(rank) * 128 + quarter * 32;
+      const int row0 = tc.m_blk * TILE_M + static_cast<int>(rank) * (TILE_M / 2) + (TALL ? half * 128 : 0) + quarter * 32;
       const uint32_t t_row = tmem_base + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = half * (TILE_N / 2); c < (half + 1) * (TILE_N / 2); c += 32, ++chunk_count) {
+      for (int c = c_begin; c < c_end; c += 32, ++chunk_count) {
         const int col = tc.n_blk * TILE_N + c;
         const bool inside = row0 < p.M && col < p.N;
         uint32_t r[32];
@@ -314,10 +335,11 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
             if (p.act == ACT_SILU) gate_chunk_train<ACT_SILU>(r, u, h);
             else if (p.act == ACT_GELU) gate_chunk_train<ACT_GELU>(r, u, h);
             else gate_chunk_train<ACT_GELU_TANH>(r, u, h);
-            // three buffers in turn: two stores lie between two uses of one
+            // the stores come in the order h, P, A: two lie between two uses of h's buffer, one between A's and the
+            // next P's use of the other, none between P's and A's
             StagedStore<OUT_DT>::template store<2>(h, stage, 0, lane, &maps.out[0], col, row0, inside);
-            StagedStore<HB200_DT_FP32>::template store<2>(u, stage + 4096, 0, lane, &maps.out[1], col, row0, inside);
-            StagedStore<HB200_DT_FP32>::template store<2>(r, stage + 8192, 0, lane, &maps.out[2], col, row0, inside);
+            StagedStore<HB200_DT_FP32>::template store<1>(u, stage + 2048, 0, lane, &maps.out[1], col, row0, inside);
+            StagedStore<HB200_DT_FP32>::template store<0>(r, stage + 2048, 0, lane, &maps.out[2], col, row0, inside);
           }
         } else {
           tmem_wait_ld();
@@ -398,7 +420,8 @@ int launch_gated_pair(const GatedMaps& maps, const GatedParams& p, DeviceCtx* ct
   constexpr int TILE_N = MODE == MODE_GATED || MODE == MODE_GATED_TRAIN ? BN / 2 : BN;
   static std::atomic<uint64_t> smem_attr_done{0};
   HB_CUDA_CHECK(set_max_dynamic_smem_once(smem_attr_done, reinterpret_cast<const void*>(kernel), L::SMEM_BYTES, device));
-  const int64_t tiles = ((p.M + static_cast<int64_t>(GG_BM) - 1) / GG_BM) * ((p.N + static_cast<int64_t>(TILE_N) - 1) / TILE_N) *
+  constexpr int64_t TILE_M = L::TALL ? 2 * GG_BM : GG_BM;
+  const int64_t tiles = ((p.M + TILE_M - 1) / TILE_M) * ((p.N + static_cast<int64_t>(TILE_N) - 1) / TILE_N) *
                         (MODE == MODE_TWIN ? 2 : (MODE == MODE_SUM_SPLIT ? p.splits : 1));
   const int pairs = static_cast<int>(tiles < ctx->num_sms / 2 ? tiles : ctx->num_sms / 2);
   HB_CUDA_CHECK(launch_pdl(kernel, static_cast<unsigned>(2 * pairs), GG_THREADS, L::SMEM_BYTES, stream, maps, p));

@@ -125,7 +125,7 @@ def grads64(x, wg, wu, dh, kind, tiniest=0.0):
 @pytest.mark.parametrize("layout", ["col", "row"])
 @pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
-@pytest.mark.parametrize("m,k,f", [(1, 8, 8), (3, 40, 24), (65, 33, 50), (130, 264, 1000), (333, 1000, 728), (512, 4096, 512), (1025, 264, 2056), (200, 520, 9000), (60, 2048, 1000)])
+@pytest.mark.parametrize("m,k,f", [(1, 8, 8), (3, 40, 24), (65, 33, 50), (130, 264, 1000), (333, 1000, 728), (512, 4096, 512), (1025, 264, 2056), (200, 520, 9000), (60, 2048, 1000), (1100, 4104, 264)])
 def test_gradients(hb, m, k, f, dtype, kind, layout):
     g = torch.Generator(device="cuda").manual_seed(m * 7 + k + f)
     x = torch.randn(m, k, generator=g, device="cuda").to(dtype).requires_grad_()
