@@ -19,22 +19,24 @@ _ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.
 
 
 def _check_gated(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str, what: str) -> int:
-    if x.dim() != 2 or w_gate.dim() != 2 or w_up.dim() != 2:
-        raise ValueError(f"{what} expects 2-D inputs, got {tuple(x.shape)}, {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
-    if w_gate.shape != w_up.shape:
-        raise ValueError(f"{what}: w_gate {tuple(w_gate.shape)} and w_up {tuple(w_up.shape)} differ in shape")
-    if x.shape[1] != w_gate.shape[0]:
-        raise ValueError(f"{what}: size mismatch, x is {tuple(x.shape)} and the weights {tuple(w_gate.shape)}")
-    if activation not in _ACTIVATIONS:
+    xs, gs, us = x.shape, w_gate.shape, w_up.shape
+    if not (len(xs) == len(gs) == len(us) == 2):
+        raise ValueError(f"{what} expects 2-D inputs, got {tuple(xs)}, {tuple(gs)} and {tuple(us)}")
+    if gs != us:
+        raise ValueError(f"{what}: w_gate {tuple(gs)} and w_up {tuple(us)} differ in shape")
+    if xs[1] != gs[0]:
+        raise ValueError(f"{what}: size mismatch, x is {tuple(xs)} and the weights {tuple(gs)}")
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"{what}: activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
-    return _ACTIVATIONS[activation]
+    return act
 
 
 def _rows_ready(t: torch.Tensor, per16: int) -> torch.Tensor:
     """``t`` itself where its rows are what the kernels read (unit column stride, 16-byte aligned), else a copy."""
     rs, cs = t.stride()
     if cs == 1 and rs % per16 == 0 and rs >= t.shape[1] and t.data_ptr() % 16 == 0:
-        return t
+        return t  # (a single row's stride counts too: it goes into a tensor map)
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -49,12 +51,15 @@ def _weights_ready(w_gate: torch.Tensor, w_up: torch.Tensor, per16: int, row_maj
     return _rows_ready(w_gate.t(), per16).t(), _rows_ready(w_up.t(), per16).t()
 
 
-def _launch(x, w_gate, w_up, out, act: int, dev: int, what: str, scales=(None, None, None), mode: int = _lib.SCALE_NONE, saved=(None, None)):
+def _launch(x, w_gate, w_up, out, act: int, dev: int, what: str, scales=None, mode: int = _lib.SCALE_NONE, saved=(None, None)):
     m, k = x.shape
+    sx = sg = su = None
+    if scales is not None:
+        sx, sg, su = scales[0].data_ptr(), scales[1].data_ptr(), scales[2].data_ptr()
     code = _lib.load().hb200_gated_gemm(
         x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), out.data_ptr(), m, out.shape[1], k, x.stride(0),
-        *w_gate.stride(), *w_up.stride(), out.stride(0), _OUT_DT[x.dtype], _OUT_DT[out.dtype], act, *scales, mode, *saved, dev,
-        _stream_ptr(dev),
+        *w_gate.stride(), *w_up.stride(), out.stride(0), _OUT_DT[x.dtype], _OUT_DT[out.dtype], act, sx, sg, su, mode, *saved,
+        dev, _stream_ptr(dev),
     )
     if code:
         _lib.raise_for(code, what)
@@ -167,25 +172,26 @@ def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
 
 
 def _gated_scales(scale_x, scale_gate, scale_up, m: int, f: int, dev: int):
-    """Validate the three scales; returns contiguous fp32 vectors and the C-ABI scale mode."""
-    scales = (scale_x, scale_gate, scale_up)
+    """Validate the three scales; returns them as contiguous fp32 tensors with the C-ABI scale mode."""
     if scale_x is None or scale_gate is None or scale_up is None:
-        if any(s is not None for s in scales):
+        if not (scale_x is None and scale_gate is None and scale_up is None):
             raise ValueError("gated_gemm: pass scale_x, scale_gate and scale_up, or none of them")
-        return (), _lib.SCALE_NONE
-    for name, t in zip(("scale_x", "scale_gate", "scale_up"), scales):
-        if t.dtype != torch.float32:
-            raise TypeError(f"gated_gemm: {name} must be a float32 tensor")
-        if t.get_device() != dev:
-            raise ValueError(f"gated_gemm: {name} must live on the inputs' device")
-    shapes = scale_x.shape, scale_gate.shape, scale_up.shape
-    if shapes[0] in ((m, 1), (m,)) and shapes[1] in ((1, f), (f,)) and shapes[2] in ((1, f), (f,)):
-        return tuple(s if s.is_contiguous() else s.contiguous() for s in scales), _lib.SCALE_ROWWISE
-    if all(s.numel() == 1 for s in scales):
+        return None, _lib.SCALE_NONE
+    scales = (scale_x, scale_gate, scale_up)
+    if not (scale_x.dtype == scale_gate.dtype == scale_up.dtype == torch.float32):
+        raise TypeError("gated_gemm: scale_x, scale_gate and scale_up must be float32 tensors")
+    if not (scale_x.get_device() == scale_gate.get_device() == scale_up.get_device() == dev):
+        raise ValueError("gated_gemm: scale_x, scale_gate and scale_up must live on the inputs' device")
+    columns = ((1, f), (f,))
+    if scale_x.shape in ((m, 1), (m,)) and scale_gate.shape in columns and scale_up.shape in columns:
+        if scale_x.is_contiguous() and scale_gate.is_contiguous() and scale_up.is_contiguous():
+            return scales, _lib.SCALE_ROWWISE
+        return tuple(s.contiguous() for s in scales), _lib.SCALE_ROWWISE
+    if scale_x.numel() == scale_gate.numel() == scale_up.numel() == 1:
         return scales, _lib.SCALE_TENSOR
     raise ValueError(
         "gated_gemm: scales must be one element each, or [M,1]/[M], [1,F]/[F] and [1,F]/[F]; got "
-        f"{tuple(shapes[0])}, {tuple(shapes[1])} and {tuple(shapes[2])} for M={m}, F={f}"
+        f"{tuple(scale_x.shape)}, {tuple(scale_gate.shape)} and {tuple(scale_up.shape)} for M={m}, F={f}"
     )
 
 
@@ -237,11 +243,9 @@ def gated_gemm(
             padded.append(wp.t())
         if mode == _lib.SCALE_ROWWISE:
             scales = (scales[0], *(torch.nn.functional.pad(s.reshape(f), (0, fp - f)) for s in scales[1:]))
-        res = x.new_empty((m, fp), dtype=out_dtype)
-        ptrs = tuple(s.data_ptr() for s in scales) or (None, None, None)
-        out.copy_(_launch(xp, *padded, res, act, dev, "gated_gemm", ptrs, mode)[:, :f])
+        res = _empty_matrix(x, m, fp, out_dtype)
+        out.copy_(_launch(xp, *padded, res, act, dev, "gated_gemm", scales, mode)[:, :f])
         return out
     x = _rows_ready(x, 16)
     w_gate, w_up = _weights_ready(w_gate, w_up, 16, False)
-    ptrs = tuple(s.data_ptr() for s in scales) or (None, None, None)
-    return _launch(x, w_gate, w_up, out, act, dev, "gated_gemm", ptrs, mode)
+    return _launch(x, w_gate, w_up, out, act, dev, "gated_gemm", scales, mode)

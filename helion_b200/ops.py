@@ -424,13 +424,16 @@ def preprocess_fp8_attention_inputs(
     return q8.reshape(bh, seq, dim), k8.reshape(bh, seq, dim), v8.reshape(bh, seq, dim).permute(0, 2, 1)
 
 
-def _row_view(t: torch.Tensor, n: int) -> torch.Tensor:
-    """``[..., N]`` as rows ``[M, N]`` of unit column stride that do not overlap (a copy only where there is no such view)."""
+def _row_view(t: torch.Tensor, n: int):
+    """``[..., N]`` as rows of unit column stride that do not overlap (a copy only where there is no such view), and
+    their stride."""
+    if t.is_contiguous():
+        return t, n
     if t.dim() != 2:
         t = t.reshape(math.prod(t.shape[:-1]), n)
     if t.stride(1) != 1 or (t.stride(0) < n and t.shape[0] > 1):
         t = t.contiguous()
-    return t
+    return t, t.stride(0) if t.shape[0] > 1 else n
 
 
 def _empty_matrix(like: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
@@ -485,13 +488,12 @@ def quantize_rows(
     n = shape[-1]
     codes = _out_rows(out, x, shape, out_dtype, "quantize_rows: `out`")
     scales = _out_rows(scale_out, x, (*shape[:-1], 1), torch.float32, "quantize_rows: `scale_out`")
-    rows = _row_view(x, n)
-    m = rows.shape[0]
+    rows, x_rs = _row_view(x, n)
+    m = scales.numel()
     if m == 0:
         return codes, scales
     code = _lib.load().hb200_quantize_rows(
-        rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, n, rows.stride(0) if m > 1 else n, n, source, target, dev,
-        _stream_ptr(dev),
+        rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, n, x_rs, n, source, target, dev, _stream_ptr(dev)
     )
     if code:
         _lib.raise_for(code, "quantize_rows")
@@ -540,22 +542,20 @@ def rms_norm_quantize(
         dev = _require_cuda(x, weight, residual)
     codes = _out_rows(out, x, shape, out_dtype, "rms_norm_quantize: `out`")
     scales = _out_rows(scale_out, x, (*shape[:-1], 1), torch.float32, "rms_norm_quantize: `scale_out`")
-    rows = _row_view(x, n)
-    m = rows.shape[0]
-    if weight.stride(0) != 1:
+    rows, x_rs = _row_view(x, n)
+    m = scales.numel()
+    if not weight.is_contiguous():
         weight = weight.contiguous()
     summed = res_ptr = sum_ptr = None
     res_rs = n
     if residual is not None:
         summed = _out_rows(residual_out, x, shape, dtype, "rms_norm_quantize: `residual_out`")
-        res = _row_view(residual, n)
-        if m > 1:
-            res_rs = res.stride(0)
+        res, res_rs = _row_view(residual, n)
         res_ptr, sum_ptr = res.data_ptr(), summed.data_ptr()
     if m > 0:
         code = _lib.load().hb200_rms_norm_quantize(
             rows.data_ptr(), res_ptr, weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), sum_ptr, m, n,
-            rows.stride(0) if m > 1 else n, res_rs, n, n, source, w_type, target, eps, dev, _stream_ptr(dev),
+            x_rs, res_rs, n, n, source, w_type, target, eps, dev, _stream_ptr(dev),
         )
         if code:
             _lib.raise_for(code, "rms_norm_quantize")
