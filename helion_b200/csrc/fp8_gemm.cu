@@ -1383,10 +1383,44 @@ int launch_gemm_16bit(const GemmArgs& a, DeviceCtx* ctx) {
 
 // ------------------------------------------------------------------------------------------------
 // Signed 8-bit integer operands through the same kernels (hb200_int8_gemm): kind::i8 instructions, int32
-// accumulators, y column-major.  The tensor pipe runs them at the e4m3 rate, so the table and its choice are the
-// same; up to 128 rows of x go to the weight-streaming kernel instead (gemm_few_rows.cu).
+// accumulators, y column-major.  The tensor pipe runs them at the e4m3 rate; up to 128 rows of x go to the
+// weight-streaming kernel instead (gemm_few_rows.cu).
 // ------------------------------------------------------------------------------------------------
 namespace {
+
+// Table row with the smallest estimated time.  A tile's K loop takes `block` microseconds per 128 of K and its epilogue
+// `drain`; rows with two accumulators overlap the one with the next tile's other, so a round of tiles takes the longer of
+// the two and one of the shorter stays exposed; the 512-row tiles (`serial`) overlap nothing.  The constants are fitted to
+// 46 random problems of 129..8192 x 256..8192 x 256..8192, every row timed in a graph: the choice is within 4 % of the
+// best row on 45 of them.  For example (rows 3 / 1 / 2 / 6 / 14 / 21, us): 5827 x 4096 x 3616 78 / 98 / 176 / 64 / 75 / 86,
+// 2331 x 5704 x 6992 114 / 147 / 205 / 96 / 82 / 78, 4062 x 1440 x 272 15.6 / 13.7 / 15.1 / 15.1 / 11.9 / 11.0.
+int select_s8_config(int64_t M, int64_t N, int64_t K, int num_sms) {
+  struct Row {
+    int cfg;
+    int64_t bm, bn;
+    bool pair, serial;
+    double block, drain;
+  };
+  const Row rows[6] = {
+      {3, 128, 256, false, false, 0.42, 5.5}, {1, 128, 128, false, false, 0.30, 3.0}, {2, 128, 64, false, false, 0.285, 1.8},
+      {6, 256, 256, true, false, 0.38, 6.0},  {14, 512, 256, true, true, 0.61, 6.2},  {21, 512, 224, true, true, 0.55, 5.6},
+  };
+  const double blocks = static_cast<double>((K + BK - 1) / BK);
+  int best = -1;
+  double best_time = 0.0;
+  for (const Row& r : rows) {
+    const int64_t tiles = ((M + r.bm - 1) / r.bm) * ((N + r.bn - 1) / r.bn);
+    const int64_t at_once = r.pair ? num_sms / 2 : num_sms;
+    const double rounds = static_cast<double>((tiles + at_once - 1) / at_once);
+    const double loop = blocks * r.block;
+    const double time = r.serial ? rounds * (loop + r.drain) : rounds * std::max(loop, r.drain) + std::min(loop, r.drain);
+    if (best < 0 || time < best_time) {
+      best = r.cfg;
+      best_time = time;
+    }
+  }
+  return best;
+}
 
 template <int OUT_DT>
 int launch_s8_row(const GemmArgs& a, DeviceCtx* ctx, const GemmConfig& c, const CUtensorMap& ta, const CUtensorMap& tb) {
@@ -1404,7 +1438,7 @@ int launch_int8_gemm(const GemmArgs& a, DeviceCtx* ctx) {
   int cfg_id = a.cfg_id;
   if (cfg_id < 0) {
     if (a.M <= kFewRowsMax) return launch_few_rows(few_rows_args(a), ctx);
-    cfg_id = gemm_select_config_nosplit(a.M, a.N, a.K, true, ctx->num_sms);
+    cfg_id = select_s8_config(a.M, a.N, a.K, ctx->num_sms);
   }
   if (cfg_id >= kNumGemmConfigs) return set_error(HB200_ERR_BAD_CONFIG, "int8_gemm: no such config");
   const GemmConfig& c = kGemmConfigs[cfg_id];
