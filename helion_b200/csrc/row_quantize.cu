@@ -36,6 +36,7 @@ struct RowQuantArgs {
   bool weight_fp32;     // else of x's type
   bool weight_vectors;  // the weight is 16-byte aligned
   bool int8;            // else e4m3
+  bool in_place;        // residual_out is x or the residual
 };
 
 struct RowQuantLaunch {
@@ -118,7 +119,7 @@ __device__ __forceinline__ void store8(typename Src<SRC_DT>::T* p, const float (
 // [from, to): where the tensor's values lie, relative to the row.  A group that hangs over its row's end, but not over the
 // tensor's, is read whole and masked (its other values are a neighbouring row's): a branch to eight single loads
 // costs the row's first and last warp a round trip to memory per tensor (1237 x 5003 fp16 with residual: 17.1 us, masked
-// 16.0 us).
+// 16.0 us).  Not where the sum overwrites x or the residual: another CTA may be writing that neighbouring row.
 template <int SRC_DT, int TIER>
 __device__ __forceinline__ void load_group(const typename Src<SRC_DT>::T* row, int64_t lo, int64_t N, int64_t from, int64_t to,
                                            float (&v)[8]) {
@@ -299,9 +300,10 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 512 : 1024) row_quantiz
 
   // x of group g, and the residual
   auto load = [&](int64_t g, float (&t)[8], float (&rv)[8]) {
-    load_group<SRC_DT, TIER>(x, first + g * 8, a.N, -row * a.x_rs, (a.M - 1 - row) * a.x_rs + a.N, t);
+    const int64_t before = a.in_place ? 0 : row, behind = a.in_place ? 0 : a.M - 1 - row;  // rows that may be read too
+    load_group<SRC_DT, TIER>(x, first + g * 8, a.N, -before * a.x_rs, behind * a.x_rs + a.N, t);
     if constexpr (MODE == 2) {
-      load_group<SRC_DT, TIER>(r, first + g * 8, a.N, -row * a.residual_rs, (a.M - 1 - row) * a.residual_rs + a.N, rv);
+      load_group<SRC_DT, TIER>(r, first + g * 8, a.N, -before * a.residual_rs, behind * a.residual_rs + a.N, rv);
     }
   };
   // s w (or x) of group g; adds to the sum of squares and the largest magnitude, writes the residual sum
@@ -622,6 +624,7 @@ int launch_row_quantize(const RowQuantCall& c, DeviceCtx* ctx, int device, cudaS
   a.eps = c.eps;
   a.weight_fp32 = c.weight_dtype == HB200_DT_FP32;
   a.weight_vectors = reinterpret_cast<uintptr_t>(c.weight) % 16 == 0;
+  a.in_place = c.residual_out != nullptr && (c.residual_out == c.x || c.residual_out == c.residual);
   a.int8 = c.out_dtype == HB200_DT_INT8;
   switch (c.src_dtype) {
     case HB200_DT_FP16:

@@ -213,7 +213,8 @@ def gated_gemm(
     three or none) are one element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of the
     weights (``[1, F]`` / ``[F]``).  One kernel, ``g`` and ``u`` in fp32, one rounding to ``out_dtype`` (fp16, bf16 or
     fp32).  Weights are best column-major (a transposed view of ``[F, K]`` storage); row-major ones are re-laid out in
-    every call.  Up to 128 rows of ``x`` run in a kernel that streams the weights.
+    every call.  Up to 128 rows of ``x`` run in a kernel that streams the weights.  The result has no gradient; ``out``
+    must not overlap the inputs.
     """
     if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float8_e4m3fn, torch.int8):
         raise TypeError(f"gated_gemm expects three float8_e4m3fn or three int8 tensors, got {x.dtype}, {w_gate.dtype} and {w_up.dtype}")

@@ -204,7 +204,8 @@ def int8_gemm(
     The int8 sibling of :func:`fp8_gemm` with its arguments: ``scale_a`` / ``scale_b`` (fp32, both or neither) are one
     element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of ``y`` (``[1, N]`` / ``[N]``), as
     :func:`quantize_rows` and :func:`rms_norm_quantize` make them.  ``y`` is best column-major (a transposed view of
-    ``[N, K]`` storage); a row-major one is re-laid out in every call.  ``K`` is below 131072.
+    ``[N, K]`` storage); a row-major one is re-laid out in every call.  ``K`` is below 131072.  The result has no
+    gradient; ``out`` must not overlap the inputs.
     """
     if x.dtype != torch.int8 or y.dtype != torch.int8:
         raise TypeError(f"int8_gemm expects int8 inputs, got {x.dtype} and {y.dtype}")
@@ -479,8 +480,8 @@ def quantize_rows(
     ``scale = max|x| / Q`` and ``code = round(x / scale)`` in fp32 with ``Q`` = 448 (``float8_e4m3fn``) or 127
     (``int8``): what :func:`fp8_gemm`, :func:`int8_gemm` and :func:`gated_gemm` take as ``x`` and its row scale.
     ``x`` is fp16, bf16 or fp32.  A row of zeros (``max|x| < 2**-100``) gets zero codes and the smallest normal
-    scale; a NaN makes its row's scale NaN, an infinity makes it infinite.  ``out`` and ``scale_out`` (contiguous)
-    take the results of a caller that keeps its buffers.
+    scale; a NaN makes its row's scale NaN, an infinity makes it infinite.  ``out`` and ``scale_out`` (contiguous, apart
+    from ``x``) take the results of a caller that keeps its buffers.  The results have no gradient.
     """
     source, target = _check_row_input(x, out_dtype, "quantize_rows")
     dev = _require_cuda(x)
@@ -518,7 +519,8 @@ def rms_norm_quantize(
     residual of the next layer.  The norm takes the fp32 sum before that rounding.  ``x`` and ``residual`` share one
     dtype (fp16, bf16, fp32); ``weight [N]`` has it too or is fp32.  ``residual_out`` may be ``x`` or ``residual``
     itself (an update in place); ``eps`` is a positive normal fp32 number; ``out``, ``scale_out`` and ``residual_out``
-    are contiguous.  A row whose sum of squares is not finite in fp32 gets a NaN scale.
+    are contiguous and overlap nothing else.  A row whose sum of squares is not finite in fp32 gets a NaN scale.  The
+    results have no gradient.
     """
     source, target = _check_row_input(x, out_dtype, "rms_norm_quantize")
     shape, dtype = x.shape, x.dtype

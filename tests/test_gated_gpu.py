@@ -122,6 +122,15 @@ def grads64(x, wg, wu, dh, kind, tiniest=0.0):
     return three(x, wg, wu, dg, du), three(*mag, dg.abs(), du.abs()), three(*mag, *off)
 
 
+def check_grads(got, x, wg, wu, dh, kind, dtype, terms):
+    """Gradients against the formula for x, weights and dh in 64 bits; terms: how many each one sums."""
+    for name, a, w, s, e, n in zip(("dx", "dw_gate", "dw_up"), got, *grads64(x, wg, wu, dh, kind, TINIEST[dtype]), terms):
+        assert a.dtype == dtype and a.shape == w.shape
+        bound = HALF_STEP[dtype] * w.abs() + (HALF_STEP[dtype] + 2.0**-20 + (n + 4) * 2.0**-24) * s + e + TINIEST[dtype]
+        off = (a.double() - w).abs() - bound
+        assert off.max().item() <= 0, f"{name}: {off.max().item()} beyond the bound"
+
+
 @pytest.mark.parametrize("layout", ["col", "row"])
 @pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
@@ -139,12 +148,7 @@ def test_gradients(hb, m, k, f, dtype, kind, layout):
     args = [t.detach().double() for t in (x, wg, wu)]
     check_forward(h.detach(), *args, kind)
     got = torch.autograd.grad(h, (x, wg, wu), dh)
-    terms = (2 * f, m, m)
-    for name, a, w, s, e, n in zip(("dx", "dw_gate", "dw_up"), got, *grads64(*args, dh.double(), kind, TINIEST[dtype]), terms):
-        assert a.dtype == dtype and a.shape == w.shape
-        bound = HALF_STEP[dtype] * w.abs() + (HALF_STEP[dtype] + 2.0**-20 + (n + 4) * 2.0**-24) * s + e + TINIEST[dtype]
-        off = (a.double() - w).abs() - bound
-        assert off.max().item() <= 0, f"{name}: {off.max().item()} beyond the bound"
+    check_grads(got, *args, dh.double(), kind, dtype, (2 * f, m, m))
 
 
 def test_formula_against_differences():
@@ -226,6 +230,29 @@ def test_extreme_pre_activations(hb):
             assert not h.isnan().any()
             dx = torch.autograd.grad(h, leaves[0], torch.full_like(h, 2.0**-120))[0]
             assert not dx.isnan().any()
+
+
+def test_offsets_beyond_31_bits(hb):
+    g = torch.Generator(device="cuda").manual_seed(14)
+    m, f = 70000, 32776
+    x, wg, wu = eight_bit(g, m, 16, torch.int8), eight_bit(g, f, 16, torch.int8).t(), eight_bit(g, f, 16, torch.int8).t()
+    s = torch.full((1,), 0.004, device="cuda")
+    out = hb.gated_gemm(x, wg, wu, scale_x=s, scale_gate=s, scale_up=s)
+    s64 = s.double()
+    for rows in (slice(0, 5), slice(m - 300, m)):
+        check_forward(out[rows], x[rows].double() * s64, wg.double() * s64, wu.double() * s64, "silu", True)
+    del out
+    xb = torch.zeros(m, 8, device="cuda", dtype=torch.bfloat16)
+    xb[-2:] = torch.randn(2, 8, generator=g, device="cuda").bfloat16()
+    wb = [torch.randn(f, 8, generator=g, device="cuda").bfloat16().t() for _ in range(2)]
+    leaves = [xb.requires_grad_(), *(w.requires_grad_() for w in wb)]
+    h = hb.gated_matmul(*leaves)
+    dh = torch.zeros_like(h)
+    dh[-2:] = 1
+    got = torch.autograd.grad(h, leaves, dh)
+    assert (got[0][:-2] == 0).all()
+    last = [xb.detach()[-2:].double(), *(w.detach().double() for w in wb), dh[-2:].double()]
+    check_grads((got[0][-2:], *got[1:]), *last, "silu", torch.bfloat16, (2 * f, 2, 2))
 
 
 def test_empty_dimensions(hb):

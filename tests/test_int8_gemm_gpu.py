@@ -101,6 +101,15 @@ def test_rows_behind_the_last_are_left_alone(hb):
         assert (store[m:] == 9).all() and (store[:, 256:] == 9).all()
 
 
+def test_offsets_beyond_31_bits(hb):
+    g = torch.Generator(device="cuda").manual_seed(14)
+    m, n = 70000, 32776
+    x, y = codes(g, m, 16), codes(g, n, 16).t()
+    out = hb.int8_gemm(x, y)
+    check(out[-300:], x[-300:], y)
+    check(out[:5], x[:5], y)
+
+
 def test_empty_dimensions(hb):
     z = lambda *s: torch.zeros(s, device="cuda", dtype=torch.int8)  # noqa: E731
     assert hb.int8_gemm(z(0, 32), z(32, 8)).shape == (0, 8) and hb.int8_gemm(z(4, 32), z(32, 0)).shape == (4, 0)

@@ -188,15 +188,41 @@ def test_rows_of_zeros_tiny_rows_and_rows_that_are_not_finite(hb):
 def test_the_first_call_of_a_process_may_be_captured(hb):
     code = """
 import torch, helion_b200 as hb
-x = torch.randn(2, 64, device="cuda")
+x = torch.randn(2, 1024, device="cuda")
+w = torch.randint(-128, 128, (2, 256, 1024), device="cuda", dtype=torch.int8)
+def calls():
+    codes, scales = hb.quantize_rows(x, out_dtype=torch.int8)
+    s = scales.new_ones(1, 256)
+    few = hb.int8_gemm(codes, w[0].t(), scale_a=scales, scale_b=s, out_dtype=torch.float32)
+    gated = hb.gated_gemm(codes, w[0].t(), w[1].t(), scale_x=scales, scale_gate=s, scale_up=s, out_dtype=torch.float32)
+    many = hb.int8_gemm(w[0], w[1].t(), out_dtype=torch.float32)
+    return codes, scales, few, gated, many
 graph = torch.cuda.CUDAGraph()
 with torch.cuda.graph(graph):
-    codes, scales = hb.quantize_rows(x)
+    got = calls()
 graph.replay()
-want = hb.quantize_rows(x)
-assert torch.equal(codes.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
+assert all(torch.equal(a, b) for a, b in zip(got, calls()))
 """
     subprocess.run([sys.executable, "-c", code], check=True, cwd=Path(__file__).resolve().parent.parent, timeout=300)
+
+
+def test_offsets_beyond_31_bits(hb):
+    """The last rows of a matrix of 2.3e9 values are what they are on their own."""
+    m, n = 70000, 32776
+    x = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16)
+    x[-3:] = torch.randn(3, n, device="cuda").bfloat16()
+    x[70] = 5.0
+    codes, scales = hb.quantize_rows(x)
+    want = hb.quantize_rows(x[-3:].clone())
+    assert torch.equal(codes[-3:].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales[-3:], want[1])
+    assert (codes[70].float() == 448).all() and scales[71].item() == pytest.approx(TINY)
+    del codes, scales
+    m, n = 140000, 16384  # many rows: through the ring
+    x = x.view(-1)[: m * n].view(m, n)
+    x[-1] = torch.randn(n, device="cuda").bfloat16()
+    codes, scales = hb.quantize_rows(x)
+    want = hb.quantize_rows(x[-1:].clone())
+    assert torch.equal(codes[-1:].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales[-1:], want[1])
 
 
 def test_empty_inputs(hb):
