@@ -376,15 +376,16 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 512 : 1024) row_quantiz
 }
 
 // ------------------------------------------------------------------------------------------------
-// Many long rows: persistent CTAs whose rows arrive in a ring of shared-memory stages by bulk copies, so that the memory
-// system stays busy while a row waits for its reduction.  (With a CTA a row, loads and reductions take turns, and the
-// registers of an SM's two to four CTAs hold too few rows in flight.)  A stage is one row of x (and one of the residual);
-// values go to registers on arrival, and the reduction's barrier hands the stage back for the row `stages` ahead.
+// Many long 16-bit rows: persistent CTAs whose rows arrive in a ring of shared-memory stages by bulk copies, so that the
+// memory system stays busy while a row waits for its reduction.  (With a CTA a row, loads and reductions take turns, and
+// the registers of an SM's two to four CTAs hold too few rows in flight.)  A stage is one row of x (and one of the
+// residual); values go to registers on arrival, and the reduction's barrier hands the stage back for the row `stages` ahead.
 //
-// Measured, bf16, a CTA a row / ring: 4096 x 14336 quantised 55.1 / 31.9 us (5.5 TB/s), with norm and residual
-// 85.1 / 68.4 us (6.0 TB/s); 8192 x 4096 quantised 27.0 / 21.1 us, with norm and residual 43.6 / 41.7 us (5.6 TB/s).
-// Below 4096 values a row the CTA-a-row form is as fast or faster (4096 x 2048 with norm 11.7 / 14.4 us), and for rows
-// that are not aligned (1237 x 5003 fp16) the ring gained nothing over it.
+// Measured, bf16, a CTA a row / ring (us; % of the copy bandwidth of 6.55 TB/s): with norm and residual 8192 x 4096
+// 44.7 / 42.2 (85 %), 4096 x 8192 51.7 / 40.8, 4096 x 14336 93.3 / 68.8 (91 %), 600 x 8192 10.0 / 9.1, but 2048 x 4096
+// 12.7 / 14.0; quantised 8192 x 4096 27.6 / 21.6 (71 %), 4096 x 14336 36.3 / 32.5 (83 %), but 600 x 8192 4.1 / 5.5.
+// With the norm alone, and for fp32 rows, whose CTAs hold twice the bytes each, it gains nothing (4096 x 8192 with norm
+// 29.7 / 32.0; fp32 4096 x 8192 with residual 70.3 / 77.5), nor for rows that are not aligned.
 // ------------------------------------------------------------------------------------------------
 constexpr int RING_MAX_STAGES = 8;
 constexpr int RING_SMEM_PER_SM = 220 * 1024;
@@ -397,7 +398,7 @@ struct RowRing {
 };
 
 template <int SRC_DT, int VPT, int MODE>
-__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) row_ring_kernel(RowQuantArgs a, RowRing ring) {
+__global__ void __launch_bounds__(VPT == 2 ? 1024 : 512) row_ring_kernel(RowQuantArgs a, RowRing ring) {
   using T = typename Src<SRC_DT>::T;
   constexpr int TENSORS = MODE == 2 ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -512,20 +513,21 @@ int launch_ring(const RowQuantArgs& a, const RowRing& ring, int ctas_per_sm, con
   return HB200_OK;
 }
 
-// The ring kernel where it applies: rows of 4096 to 16384 values, enough of them that its CTAs loop, at least two in
-// shared memory.  Returns 1 where it does not.
+// The ring kernel where it applies (see its measurements): rows of 4096 to 16384 values, enough of them that its CTAs loop.
+// Returns 1 where it does not.
 template <int SRC_DT, int MODE>
 int try_ring(const RowQuantArgs& a, const RowQuantLaunch& l) {
   if (l.M < 4ll * l.ctx->num_sms || a.N < 4096 || a.N > 16384) return 1;
+  const int64_t values = l.M * a.N;
+  if (MODE == 2 ? a.N < 8192 && values < (1 << 24) : values < (1 << 25)) return 1;
   RowRing ring;
   ring.M = l.M;
   ring.status = l.ctx->status_dev;
-  ring.row_bytes = static_cast<int>(a.N) * static_cast<int>(sizeof(typename Src<SRC_DT>::T));
+  ring.row_bytes = static_cast<int>(a.N) * 2;
   // as many CTAs an SM as have two stages each: 4 of 256 to 512 threads, 2 of up to 512, 1 of up to 1024
   for (int ctas = a.N <= 8192 ? 4 : 2; ctas >= 1; ctas /= 2) {
     ring.stages = std::min(RING_MAX_STAGES, (RING_SMEM_PER_SM / ctas - 2048) / (ring.row_bytes * (MODE == 2 ? 2 : 1)));
     if (ring.stages < 2) continue;
-    if (ctas == 1 && a.N <= 8192) return launch_ring<SRC_DT, 1, MODE>(a, ring, ctas, l);
     return ctas == 2 && a.N > 8192 ? launch_ring<SRC_DT, 4, MODE>(a, ring, ctas, l) : launch_ring<SRC_DT, 2, MODE>(a, ring, ctas, l);
   }
   return 1;
@@ -544,7 +546,7 @@ int launch_row_size(const RowQuantArgs& a, const RowQuantLaunch& l) {
   const int vpt = groups <= 512 ? 1 : (groups <= 1024 ? 2 : 4);
   const int threads = static_cast<int>(std::min<int64_t>(((groups + vpt - 1) / vpt + 31) / 32 * 32, 1024));
   if constexpr (TIER != ROW_SCALAR) {
-    if constexpr (TIER == ROW_ALIGNED) {
+    if constexpr (TIER == ROW_ALIGNED && MODE != 1 && SRC_DT != HB200_DT_FP32) {
       const int rc = try_ring<SRC_DT, MODE>(a, l);
       if (rc <= 0) return rc;
     }

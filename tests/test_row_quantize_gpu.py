@@ -55,7 +55,7 @@ def norm64(x, weight, residual, eps):
 @pytest.mark.parametrize("out_dtype", [E4M3, torch.int8], ids=["e4m3", "int8"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("m,n", [(1, 1), (3, 7), (1, 8), (5, 64), (2, 4096), (3, 4099), (33, 5003), (2, 8200), (2, 14336), (2, 32768), (2, 32761), (3, 40000), (2, 50001),
-                                 (592, 1024), (1700, 1031), (900, 4096), (601, 5003), (777, 9000), (650, 14336), (593, 16377), (600, 16384)])
+                                 (592, 1024), (1700, 1031), (900, 4096), (601, 5003), (777, 9000), (650, 14336), (593, 16377), (600, 16384), (2401, 14336), (8200, 4096)])
 def test_quantize_rows(hb, m, n, dtype, out_dtype):
     g = torch.Generator(device="cuda").manual_seed(m * 100003 + n)
     x = (torch.randn(m, n, generator=g, device="cuda") * 3.0).to(dtype)
@@ -69,7 +69,7 @@ def test_quantize_rows(hb, m, n, dtype, out_dtype):
 @pytest.mark.parametrize("with_residual", [True, False], ids=["residual", "plain"])
 @pytest.mark.parametrize("out_dtype", [E4M3, torch.int8], ids=["e4m3", "int8"])
 @pytest.mark.parametrize("dtype,w_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16), (torch.float32, torch.float32)])
-@pytest.mark.parametrize("m,n", [(1, 1), (2, 9), (1, 4096), (7, 5003), (2, 14336), (2, 24576), (2, 40001), (1190, 1031), (900, 4096), (601, 5003), (650, 14336), (593, 16377), (600, 16384)])
+@pytest.mark.parametrize("m,n", [(1, 1), (2, 9), (1, 4096), (7, 5003), (2, 14336), (2, 24576), (2, 40001), (1190, 1031), (900, 4096), (601, 5003), (601, 8192), (650, 14336), (593, 16377), (600, 16384), (4099, 4096)])
 def test_rms_norm_quantize(hb, m, n, dtype, w_dtype, out_dtype, with_residual):
     g = torch.Generator(device="cuda").manual_seed(m * 100003 + n + 1)
     x = torch.randn(m, n, generator=g, device="cuda").to(dtype)
@@ -106,7 +106,7 @@ def test_leading_dimensions_and_given_buffers(hb):
             assert torch.equal(a.reshape(-1).view(torch.uint8), b.reshape(-1).view(torch.uint8))
 
 
-@pytest.mark.parametrize("m,n", [(3, 40003), (3, 520), (3, 77), (1500, 1031), (1500, 4096)])
+@pytest.mark.parametrize("m,n", [(3, 40003), (3, 520), (3, 77), (1500, 1031), (1500, 4096), (700, 8200)])
 def test_in_place_on_rows_of_every_kind(hb, m, n):
     """Rows read twice (n > 32768), whole and odd, few and many: the sum overwrites an input that is still being read."""
     g = torch.Generator(device="cuda").manual_seed(n)
@@ -137,7 +137,8 @@ def test_strided_and_offset_rows(hb):
     # many rows with strides and offsets
     big = torch.randn(700, 2100, generator=g, device="cuda").bfloat16()
     w = torch.rand(2100, generator=g, device="cuda")
-    for x, r, wt in ((big[:, 8:2056], big[:, 0:2048], w[:2048]), (big[:, 3:2052], big[:, 11:2060], w[:2049]), (big[:, 3:2052], big[:, 4:2053], w[:2049])):
+    for x, r, wt in ((big.view(175, -1)[:, 8:8200].repeat(4, 1)[:, :8192], big.view(175, -1)[:, :8192].repeat(4, 1), torch.rand(8192, generator=g, device="cuda")),
+                     (big[:, 8:2056], big[:, 0:2048], w[:2048]), (big[:, 3:2052], big[:, 11:2060], w[:2049]), (big[:, 3:2052], big[:, 4:2053], w[:2049])):
         got = hb.rms_norm_quantize(x, wt, residual=r)
         check_codes(*got[:2], norm64(x, wt, r, 1e-6)[1])  # the order of a row's sum goes by its layout: not the same bits
         assert torch.equal(got[2], (x.float() + r.float()).bfloat16())
