@@ -403,14 +403,16 @@ inline int gated_out_map_layers(CUtensorMap* map, void* base, int64_t m, int64_t
   return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Whether 128-column tiles finish earlier than 256-column ones: rounds of tiles over the CTA pairs times a tile's
-// length, in which the narrow tile reads 3/4 of the operand bytes for half the products.
+// Whether 128-column tiles finish earlier than 256-column ones: by the rounds of tiles over the CTA pairs.  A round of narrow
+// tiles was measured at 0.83 to 0.91 of a round of wide ones (they read 3/4 of the operand bytes for half the products:
+// bf16 forward 1327 x 1312 x 5784 69 us in 8 rounds against 40 us in 4), so they pay where the rounds are the same
+// (222 x 480 x 400 7.2 against 8.3 us).
 inline bool gated_narrow_tiles(int64_t m, int64_t columns, int products, int num_sms) {
   const int64_t pairs = num_sms / 2;
   const int64_t m_tiles = (m + GG_BM - 1) / GG_BM;
   const int64_t wide = (products * m_tiles * ((columns + 255) / 256) + pairs - 1) / pairs;
   const int64_t narrow = (products * m_tiles * ((columns + 127) / 128) + pairs - 1) / pairs;
-  return narrow * 0.6 < wide * 1.0;
+  return narrow * 0.85 < wide * 1.0;
 }
 
 template <int KIND, bool A_MN, bool B_MN, int BN, int MODE, int OUT_DT>
