@@ -738,8 +738,8 @@ static int row_quantize_impl(const char* what, const RowQuantCall& c, int device
   if (c.weight_dtype != c.src_dtype && c.weight_dtype != HB200_DT_FP32) {
     return set_error(HB200_ERR_BAD_DTYPE, name + ": weight_dtype must be src_dtype or FP32");
   }
-  if (c.M < 1 || c.N < 1 || c.M > INT32_MAX || c.N > INT32_MAX) {
-    return set_error(HB200_ERR_BAD_SHAPE, name + ": M and N must be in [1, 2^31)");
+  if (c.M < 1 || c.N < 1 || c.M > INT32_MAX || c.N > (1 << 30)) {
+    return set_error(HB200_ERR_BAD_SHAPE, name + ": M must be in [1, 2^31) and N in [1, 2^30]");
   }
   if (c.x == nullptr || c.codes == nullptr || c.scales == nullptr) return set_error(HB200_ERR_ALIGN, name + ": null pointer");
   if ((c.residual == nullptr) != (c.residual_out == nullptr)) {

@@ -121,7 +121,7 @@ __device__ __forceinline__ void store8(typename Src<SRC_DT>::T* p, const float (
 // costs the row's first and last warp a round trip to memory per tensor (1237 x 5003 fp16 with residual: 17.1 us, masked
 // 16.0 us).  Not where the sum overwrites x or the residual: another CTA may be writing that neighbouring row.
 template <int SRC_DT, int TIER>
-__device__ __forceinline__ void load_group(const typename Src<SRC_DT>::T* row, int64_t lo, int64_t N, int64_t from, int64_t to,
+__device__ __forceinline__ void load_group(const typename Src<SRC_DT>::T* row, int lo, int N, int from, int to,
                                            float (&v)[8]) {
   if (TIER == ROW_ALIGNED || (TIER == ROW_PHASED && lo >= from && lo + 8 <= to)) {
     load8<SRC_DT>(row + lo, v);
@@ -169,10 +169,10 @@ __device__ __forceinline__ void load8_shifted(const typename Src<DT>::T* aligned
 // of the weight begins: two vectors and a shift instead of eight loads (1237 x 5003 fp16 with residual: 16.0 us, with the
 // eight loads, as an fp32 weight has them, 18.9 us).
 template <int W_DT, int TIER>
-__device__ __forceinline__ void load_weight_as(const void* weight, int64_t lo, int phase, int64_t N, bool vectors, float (&v)[8]) {
+__device__ __forceinline__ void load_weight_as(const void* weight, int lo, int phase, int N, bool vectors, float (&v)[8]) {
   const auto* w = reinterpret_cast<const typename Src<W_DT>::T*>(weight);
   if constexpr (TIER == ROW_PHASED && W_DT != HB200_DT_FP32) {
-    const int64_t up = lo + phase;  // a multiple of 8
+    const int up = lo + phase;  // a multiple of 8
     if (vectors && up + 8 <= N) {
       if (phase == 0) load8<W_DT, true>(w + lo, v);
       else load8_shifted<W_DT>(w + up, up > 0, 8 - phase, v);
@@ -188,9 +188,9 @@ __device__ __forceinline__ void load_weight_as(const void* weight, int64_t lo, i
 }
 
 template <int SRC_DT, int TIER>
-__device__ __forceinline__ void load_weight(const RowQuantArgs& a, int64_t lo, int phase, float (&v)[8]) {
-  if (SRC_DT != HB200_DT_FP32 && a.weight_fp32) load_weight_as<HB200_DT_FP32, TIER>(a.weight, lo, phase, a.N, false, v);
-  else load_weight_as<SRC_DT, TIER>(a.weight, lo, phase, a.N, a.weight_vectors, v);
+__device__ __forceinline__ void load_weight(const RowQuantArgs& a, int lo, int phase, float (&v)[8]) {
+  if (SRC_DT != HB200_DT_FP32 && a.weight_fp32) load_weight_as<HB200_DT_FP32, TIER>(a.weight, lo, phase, static_cast<int>(a.N), false, v);
+  else load_weight_as<SRC_DT, TIER>(a.weight, lo, phase, static_cast<int>(a.N), a.weight_vectors, v);
 }
 
 // Bytes [0, size) of global memory, 16-byte aligned and whole 16-byte pieces, to shared memory.
@@ -201,7 +201,7 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 }
 
 template <int SRC_DT, int TIER>
-__device__ __forceinline__ void store_group(typename Src<SRC_DT>::T* row, int64_t lo, int64_t N, const float (&v)[8]) {
+__device__ __forceinline__ void store_group(typename Src<SRC_DT>::T* row, int lo, int N, const float (&v)[8]) {
   if (TIER == ROW_ALIGNED || (TIER == ROW_PHASED && lo >= 0 && lo + 8 <= N)) {
     store8<SRC_DT>(row + lo, v);
   } else {
@@ -221,7 +221,7 @@ __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, bo
 }
 
 template <int TIER>
-__device__ __forceinline__ void store_codes(uint8_t* row, int64_t lo, int64_t N, const float (&t)[8], float f, bool int8) {
+__device__ __forceinline__ void store_codes(uint8_t* row, int lo, int N, const float (&t)[8], float f, bool int8) {
   const uint32_t a = code4(t[0] * f, t[1] * f, t[2] * f, t[3] * f, int8);
   const uint32_t b = code4(t[4] * f, t[5] * f, t[6] * f, t[7] * f, int8);
   if (TIER == ROW_ALIGNED || (TIER == ROW_PHASED && lo >= 0 && lo + 8 <= N)) {
@@ -281,7 +281,7 @@ __device__ __forceinline__ void warp_reduce(float& sum, uint32_t& top) {
 // VPT groups of 8 values a thread (0: any number, the row is read twice).  MODE 0: quantise; 1: norm first;
 // 2: norm with the residual's addition.
 template <int SRC_DT, int VPT, int MODE, int TIER>
-__global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 512 : 1024) row_quantize_kernel(RowQuantArgs a) {
+__global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
   using T = typename Src<SRC_DT>::T;
   constexpr int HELD = VPT > 0 ? VPT : 1;
   __shared__ float red_sum[32];
@@ -292,29 +292,31 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 512 : 1024) row_quantiz
   T* s_out = MODE == 2 ? reinterpret_cast<T*>(a.residual_out) + row * a.residual_out_rs : nullptr;
   uint8_t* codes = reinterpret_cast<uint8_t*>(a.codes) + row * a.codes_rs;
   // first value of group 0: at or before the row's start
-  const int64_t first = TIER == ROW_PHASED ? -static_cast<int64_t>((reinterpret_cast<uintptr_t>(codes)) & 7u) : 0;
-  const int64_t groups = (a.N - first + 7) / 8;
+  const int N = static_cast<int>(a.N);
+  const int first = TIER == ROW_PHASED ? -static_cast<int>(reinterpret_cast<uintptr_t>(codes) & 7u) : 0;
+  const int groups = (N - first + 7) / 8;
+  // how far outside the row its tensors go on, up to a group: rows that may be read too
+  auto reach = [&](int64_t rows, int64_t rs) { return a.in_place ? 0 : static_cast<int>(min(rows * rs, int64_t(8))); };
+  const int x_before = reach(row, a.x_rs), x_behind = reach(a.M - 1 - row, a.x_rs);
+  const int r_before = reach(row, a.residual_rs), r_behind = reach(a.M - 1 - row, a.residual_rs);
 
   pdl_wait();
   pdl_launch_dependents();
 
   // x of group g, and the residual
-  auto load = [&](int64_t g, float (&t)[8], float (&rv)[8]) {
-    const int64_t before = a.in_place ? 0 : row, behind = a.in_place ? 0 : a.M - 1 - row;  // rows that may be read too
-    load_group<SRC_DT, TIER>(x, first + g * 8, a.N, -before * a.x_rs, behind * a.x_rs + a.N, t);
-    if constexpr (MODE == 2) {
-      load_group<SRC_DT, TIER>(r, first + g * 8, a.N, -before * a.residual_rs, behind * a.residual_rs + a.N, rv);
-    }
+  auto load = [&](int g, float (&t)[8], float (&rv)[8]) {
+    load_group<SRC_DT, TIER>(x, first + g * 8, N, -x_before, N + x_behind, t);
+    if constexpr (MODE == 2) load_group<SRC_DT, TIER>(r, first + g * 8, N, -r_before, N + r_behind, rv);
   };
   // s w (or x) of group g; adds to the sum of squares and the largest magnitude, writes the residual sum
-  auto take = [&](int64_t g, float (&t)[8], const float (&rv)[8], float& sum, uint32_t& top, bool write_sum) {
-    const int64_t lo = first + g * 8;
+  auto take = [&](int g, float (&t)[8], const float (&rv)[8], float& sum, uint32_t& top, bool write_sum) {
+    const int lo = first + g * 8;
     float wv[8];
-    if constexpr (MODE != 0) load_weight<SRC_DT, TIER>(a, lo, static_cast<int>(-first), wv);
+    if constexpr (MODE != 0) load_weight<SRC_DT, TIER>(a, lo, -first, wv);
     if constexpr (MODE == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] += rv[i];
-      if (write_sum) store_group<SRC_DT, TIER>(s_out, lo, a.N, t);
+      if (write_sum) store_group<SRC_DT, TIER>(s_out, lo, N, t);
     }
     take_group<MODE>(t, wv, sum, top);
   };
@@ -327,16 +329,16 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 512 : 1024) row_quantiz
     // cannot move a load over one
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t g = threadIdx.x + static_cast<int64_t>(v) * blockDim.x;
+      const int g = threadIdx.x + v * blockDim.x;
       if (g < groups) load(g, t[v], rv[v]);
     }
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t g = threadIdx.x + static_cast<int64_t>(v) * blockDim.x;
+      const int g = threadIdx.x + v * blockDim.x;
       if (g < groups) take(g, t[v], rv[v], sum, top, true);
     }
   } else {
-    for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) {
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
       load(g, t[0], rv[0]);
       take(g, t[0], rv[0], sum, top, false);
     }
@@ -361,16 +363,16 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 512 : 1024) row_quantiz
   if constexpr (VPT > 0) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t g = threadIdx.x + static_cast<int64_t>(v) * blockDim.x;
-      if (g < groups) store_codes<TIER>(codes, first + g * 8, a.N, t[v], f, a.int8);
+      const int g = threadIdx.x + v * blockDim.x;
+      if (g < groups) store_codes<TIER>(codes, first + g * 8, N, t[v], f, a.int8);
     }
   } else {
-    for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) {
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
       float s2 = 0.0f;
       uint32_t t2 = 0;
       load(g, t[0], rv[0]);
       take(g, t[0], rv[0], s2, t2, true);
-      store_codes<TIER>(codes, first + g * 8, a.N, t[0], f, a.int8);
+      store_codes<TIER>(codes, first + g * 8, N, t[0], f, a.int8);
     }
   }
 }
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(VPT == 2 ? 1024 : 512) row_ring_kernel(RowQuan
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int g = threadIdx.x + v * blockDim.x;
-      if (g < groups) store_codes<ROW_ALIGNED>(codes, g * 8, a.N, t[v], f, a.int8);
+      if (g < groups) store_codes<ROW_ALIGNED>(codes, g * 8, 0, t[v], f, a.int8);
     }
     turn ^= 1u;
     if (++s == ring.stages) {
@@ -543,7 +545,12 @@ int launch_row(const RowQuantArgs& a, const RowQuantLaunch& l, int threads) {
 template <int SRC_DT, int MODE, int TIER>
 int launch_row_size(const RowQuantArgs& a, const RowQuantLaunch& l) {
   const int64_t groups = (a.N + (TIER == ROW_PHASED ? 7 : 0) + 7) / 8;  // a phase adds a group at most
-  const int vpt = groups <= 512 ? 1 : (groups <= 1024 ? 2 : 4);
+  // CTAs of up to 1024 threads, rather than 512, where a row's own latency counts: rows that have an SM each (one row of
+  // 14336 bf16 with residual 4.6 / 3.6 us, quantised 2.5 / 2.2 us), and odd rows with a residual, whose masks and
+  // shifts are most of their time (1237 x 5003 15.5 / 14.7 us, 4096 x 4099 47.0 / 38.5 us).  Elsewhere the smaller ones hold
+  // more rows a SM (1237 x 8192 quantised 7.8 / 10.5 us).
+  const bool wide = l.M <= l.ctx->num_sms || (TIER == ROW_PHASED && MODE == 2 && groups <= 1024);
+  const int vpt = groups <= (wide ? 1024 : 512) ? 1 : (groups <= (wide ? 2048 : 1024) ? 2 : 4);
   const int threads = static_cast<int>(std::min<int64_t>(((groups + vpt - 1) / vpt + 31) / 32 * 32, 1024));
   if constexpr (TIER != ROW_SCALAR) {
     if constexpr (TIER == ROW_ALIGNED && MODE != 1 && SRC_DT != HB200_DT_FP32) {

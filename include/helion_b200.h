@@ -254,7 +254,7 @@ HB200_API size_t hb200_gated_gemm_backward_workspace_bytes(int64_t M, int64_t F,
  * HB200_SCALE_ROWWISE.  The reference has no counterpart (its fp8 example casts without scales,
  * examples/fp8_gemm.py:60-75).
  *   x: src_dtype FP16, BF16 or FP32, row stride x_rs >= N elements, aligned to its element size;
- *   codes: E4M3 or INT8 bytes, row stride codes_rs >= N;  scales: M floats;  N >= 1, any M >= 1.
+ *   codes: E4M3 or INT8 bytes, row stride codes_rs >= N;  scales: M floats;  M >= 1, N in [1, 2^30].
  * Aligned rows (16 bytes, N a multiple of 8) and rows that all start at the same place modulo 8 elements are read
  * with wide loads; other layouts element by element.
  * A row whose max|x| is below 2^-100 gets codes of zero and the scale FLT_MIN.  A NaN in a row makes its scale NaN;

@@ -45,7 +45,7 @@ def _call(lib, fn="norm", M=4, N=32, x_rs=32, res_rs=32, c_rs=32, so_rs=32, src=
 
 @pytest.mark.parametrize("change,code", [
     ({"src": _lib.DT_E4M3}, _lib.ERR_BAD_DTYPE), ({"od": _lib.DT_BF16}, _lib.ERR_BAD_DTYPE), ({"wd": _lib.DT_FP16}, _lib.ERR_BAD_DTYPE),
-    ({"M": 0}, _lib.ERR_BAD_SHAPE), ({"N": 0}, _lib.ERR_BAD_SHAPE), ({"M": 1 << 31}, _lib.ERR_BAD_SHAPE),
+    ({"M": 0}, _lib.ERR_BAD_SHAPE), ({"N": 0}, _lib.ERR_BAD_SHAPE), ({"M": 1 << 31}, _lib.ERR_BAD_SHAPE), ({"N": (1 << 30) + 1}, _lib.ERR_BAD_SHAPE),
     ({"x_rs": 31}, _lib.ERR_BAD_STRIDE), ({"c_rs": 31}, _lib.ERR_BAD_STRIDE), ({"res_rs": 0}, _lib.ERR_BAD_STRIDE), ({"so_rs": 16}, _lib.ERR_BAD_STRIDE),
     ({"x": 257}, _lib.ERR_ALIGN), ({"res": 513}, _lib.ERR_ALIGN), ({"w": 1025}, _lib.ERR_ALIGN), ({"so": 8193}, _lib.ERR_ALIGN), ({"scales": 4098}, _lib.ERR_ALIGN),
     ({"x": None}, _lib.ERR_ALIGN), ({"w": None}, _lib.ERR_ALIGN), ({"codes": None}, _lib.ERR_ALIGN), ({"res": None}, _lib.ERR_ALIGN), ({"so": None}, _lib.ERR_ALIGN),
