@@ -220,10 +220,24 @@ __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, bo
   return __byte_perm(lo, hi, 0x5410);
 }
 
-template <int TIER>
-__device__ __forceinline__ void store_codes(uint8_t* row, int lo, int N, const float (&t)[8], float f, bool int8) {
-  const uint32_t a = code4(t[0] * f, t[1] * f, t[2] * f, t[3] * f, int8);
-  const uint32_t b = code4(t[4] * f, t[5] * f, t[6] * f, t[7] * f, int8);
+__device__ __forceinline__ void set_pair(float (&v)[8], int i, uint64_t pair) {
+  uint32_t a, b;
+  unpack2(pair, a, b);
+  v[2 * i] = __uint_as_float(a);
+  v[2 * i + 1] = __uint_as_float(b);
+}
+
+template <int TIER, int MODE>
+__device__ __forceinline__ void store_codes(uint8_t* row, int lo, int N, const float (&t)[8], float2 f, bool int8) {
+  float v[8];
+  const uint64_t hi = pack2f(f.x, f.x), lo2 = pack2f(f.y, f.y);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t t2 = pack2f(t[2 * i], t[2 * i + 1]);
+    set_pair(v, i, MODE == 0 ? fmul2(t2, hi) : ffma2(t2, hi, fmul2(t2, lo2)));
+  }
+  const uint32_t a = code4(v[0], v[1], v[2], v[3], int8);
+  const uint32_t b = code4(v[4], v[5], v[6], v[7], int8);
   if (TIER == ROW_ALIGNED || (TIER == ROW_PHASED && lo >= 0 && lo + 8 <= N)) {
     *reinterpret_cast<uint2*>(row + lo) = make_uint2(a, b);
   } else {
@@ -234,9 +248,11 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int lo, int N, const f
   }
 }
 
-// One row's factor for the codes, and its scale.
+// One row's factor Q / max for the codes, as a sum of two floats, and its scale.  Products of few bits often lie exactly between
+// two codes; the factor's own rounding would decide these ties by chance (8192 x 4096 bf16 with residual: 104 codes of 33.6
+// million differed from the exact ones, with two floats none).  Without the norm one float was as exact (none of 58.7 million).
 template <int MODE>
-__device__ __forceinline__ float row_factor(const RowQuantArgs& a, float sum, uint32_t top, float& scale) {
+__device__ __forceinline__ float2 row_factor(const RowQuantArgs& a, float sum, uint32_t top, float& scale) {
   const float Q = a.int8 ? 127.0f : 448.0f;
   constexpr float kTiny = 1.17549435e-38f;
   const float amax = __uint_as_float(top);
@@ -251,22 +267,35 @@ __device__ __forceinline__ float row_factor(const RowQuantArgs& a, float sum, ui
     scale = kTiny;
     f = 0.0f;
   }
-  return f;
+  return make_float2(f, MODE != 0 && f > 0.0f ? fmaf(-f, amax, Q) * (f / Q) : 0.0f);
 }
 
-// Eight values of s w (or x) into the row's sum of squares and largest magnitude; t holds s (or x) on entry.
+// t += r, two values an instruction (the kernels issue close to what an SM can where rows come fast).
+__device__ __forceinline__ void add_group(float (&t)[8], const float (&r)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) set_pair(t, i, fadd2(pack2f(t[2 * i], t[2 * i + 1]), pack2f(r[2 * i], r[2 * i + 1])));
+}
+
+// Eight values of s w (or x) into the row's sum of squares (as two sums) and largest magnitude; t holds s (or x) on entry.
 template <int MODE>
-__device__ __forceinline__ void take_group(float (&t)[8], const float (&w)[8], float& sum, uint32_t& top) {
+__device__ __forceinline__ void take_group(float (&t)[8], const float (&w)[8], uint64_t& sum2, uint32_t& top) {
   if constexpr (MODE != 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum = fmaf(t[i], t[i], sum);
-      t[i] *= w[i];
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t t2 = pack2f(t[2 * i], t[2 * i + 1]);
+      sum2 = ffma2(t2, t2, sum2);
+      set_pair(t, i, fmul2(t2, pack2f(w[2 * i], w[2 * i + 1])));
     }
   }
   // magnitudes compared as bit patterns: a NaN is larger than everything and is not lost
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(t[i]) & kF32AbsMask);
+}
+
+__device__ __forceinline__ float both(uint64_t sum2) {
+  uint32_t a, b;
+  unpack2(sum2, a, b);
+  return __uint_as_float(a) + __uint_as_float(b);
 }
 
 template <int MODE>
@@ -309,20 +338,19 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
     if constexpr (MODE == 2) load_group<SRC_DT, TIER>(r, first + g * 8, N, -r_before, N + r_behind, rv);
   };
   // s w (or x) of group g; adds to the sum of squares and the largest magnitude, writes the residual sum
-  auto take = [&](int g, float (&t)[8], const float (&rv)[8], float& sum, uint32_t& top, bool write_sum) {
+  auto take = [&](int g, float (&t)[8], const float (&rv)[8], uint64_t& sum2, uint32_t& top, bool write_sum) {
     const int lo = first + g * 8;
     float wv[8];
     if constexpr (MODE != 0) load_weight<SRC_DT, TIER>(a, lo, -first, wv);
     if constexpr (MODE == 2) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] += rv[i];
+      add_group(t, rv);
       if (write_sum) store_group<SRC_DT, TIER>(s_out, lo, N, t);
     }
-    take_group<MODE>(t, wv, sum, top);
+    take_group<MODE>(t, wv, sum2, top);
   };
 
   float t[HELD][8], rv[HELD][8];
-  float sum = 0.0f;
+  uint64_t sum2 = pack2f(0.0f, 0.0f);
   uint32_t top = 0;
   if constexpr (VPT > 0) {
     // all of a thread's loads before its first store: a store may be to x or the residual itself, so the compiler
@@ -335,16 +363,17 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int g = threadIdx.x + v * blockDim.x;
-      if (g < groups) take(g, t[v], rv[v], sum, top, true);
+      if (g < groups) take(g, t[v], rv[v], sum2, top, true);
     }
   } else {
     for (int g = threadIdx.x; g < groups; g += blockDim.x) {
       load(g, t[0], rv[0]);
-      take(g, t[0], rv[0], sum, top, false);
+      take(g, t[0], rv[0], sum2, top, false);
     }
   }
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  float sum = both(sum2);
   warp_reduce<MODE>(sum, top);
   if (warps > 1) {
     if (lane == 0) {
@@ -357,22 +386,22 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
     warp_reduce<MODE>(sum, top);
   }
   float scale;
-  const float f = row_factor<MODE>(a, sum, top, scale);
+  const float2 f = row_factor<MODE>(a, sum, top, scale);
   if (threadIdx.x == 0) a.scales[row] = scale;
 
   if constexpr (VPT > 0) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int g = threadIdx.x + v * blockDim.x;
-      if (g < groups) store_codes<TIER>(codes, first + g * 8, N, t[v], f, a.int8);
+      if (g < groups) store_codes<TIER, MODE>(codes, first + g * 8, N, t[v], f, a.int8);
     }
   } else {
     for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-      float s2 = 0.0f;
+      uint64_t s2 = pack2f(0.0f, 0.0f);
       uint32_t t2 = 0;
       load(g, t[0], rv[0]);
       take(g, t[0], rv[0], s2, t2, true);
-      store_codes<TIER>(codes, first + g * 8, N, t[0], f, a.int8);
+      store_codes<TIER, MODE>(codes, first + g * 8, N, t[0], f, a.int8);
     }
   }
 }
@@ -444,7 +473,7 @@ __global__ void __launch_bounds__(VPT == 2 ? 1024 : 512) row_ring_kernel(RowQuan
     const T* sx = reinterpret_cast<const T*>(smem + s * TENSORS * ring.row_bytes);
     const bool ok = mbar_wait(&full[s], ph, wctx, SITE_ROWS_FULL);
     float t[VPT][8];
-    float sum = 0.0f;
+    uint64_t sum2 = pack2f(0.0f, 0.0f);
     uint32_t top = 0;
     if (ok) {
 #pragma unroll
@@ -455,16 +484,16 @@ __global__ void __launch_bounds__(VPT == 2 ? 1024 : 512) row_ring_kernel(RowQuan
           if constexpr (MODE == 2) {
             float rv[8];
             load8<SRC_DT>(sx + ring.row_bytes / sizeof(T) + g * 8, rv);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t[v][i] += rv[i];
+            add_group(t[v], rv);
             store8<SRC_DT>(reinterpret_cast<T*>(a.residual_out) + row * a.residual_out_rs + g * 8, t[v]);
           }
           float wv[8];
           if constexpr (MODE != 0) load_weight<SRC_DT, ROW_ALIGNED>(a, g * 8, 0, wv);
-          take_group<MODE>(t[v], wv, sum, top);
+          take_group<MODE>(t[v], wv, sum2, top);
         }
       }
     }
+    float sum = both(sum2);
     warp_reduce<MODE>(sum, top);
     if (lane == 0) {
       red_sum[turn][warp] = sum;
@@ -477,13 +506,13 @@ __global__ void __launch_bounds__(VPT == 2 ? 1024 : 512) row_ring_kernel(RowQuan
     top = lane < warps ? red_max[turn][lane] : 0u;
     warp_reduce<MODE>(sum, top);
     float scale;
-    const float f = row_factor<MODE>(a, sum, top, scale);
+    const float2 f = row_factor<MODE>(a, sum, top, scale);
     if (threadIdx.x == 0) a.scales[row] = scale;
     uint8_t* codes = reinterpret_cast<uint8_t*>(a.codes) + row * a.codes_rs;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int g = threadIdx.x + v * blockDim.x;
-      if (g < groups) store_codes<ROW_ALIGNED>(codes, g * 8, 0, t[v], f, a.int8);
+      if (g < groups) store_codes<ROW_ALIGNED, MODE>(codes, g * 8, 0, t[v], f, a.int8);
     }
     turn ^= 1u;
     if (++s == ring.stages) {
