@@ -1383,8 +1383,8 @@ int launch_gemm_16bit(const GemmArgs& a, DeviceCtx* ctx) {
 
 // ------------------------------------------------------------------------------------------------
 // Signed 8-bit integer operands through the same kernels (hb200_int8_gemm): kind::i8 instructions, int32
-// accumulators, y column-major.  The tensor pipe runs them at the e4m3 rate; up to 128 rows of x go to the
-// weight-streaming kernel instead (gemm_few_rows.cu).
+// accumulators, y column-major.  The tensor pipe runs them at the e4m3 rate; up to 128 rows of x, and more where the columns
+// are few and K long, go to the weight-streaming kernel instead (gemm_few_rows.cu).
 // ------------------------------------------------------------------------------------------------
 namespace {
 
@@ -1394,7 +1394,7 @@ namespace {
 // 46 random problems of 129..8192 x 256..8192 x 256..8192, every row timed in a graph: the choice is within 4 % of the
 // best row on 45 of them.  For example (rows 3 / 1 / 2 / 6 / 14 / 21, us): 5827 x 4096 x 3616 78 / 98 / 176 / 64 / 75 / 86,
 // 2331 x 5704 x 6992 114 / 147 / 205 / 96 / 82 / 78, 4062 x 1440 x 272 15.6 / 13.7 / 15.1 / 15.1 / 11.9 / 11.0.
-int select_s8_config(int64_t M, int64_t N, int64_t K, int num_sms) {
+int select_s8_config(int64_t M, int64_t N, int64_t K, int num_sms, double* estimate) {
   struct Row {
     int cfg;
     int64_t bm, bn;
@@ -1419,7 +1419,18 @@ int select_s8_config(int64_t M, int64_t N, int64_t K, int num_sms) {
       best_time = time;
     }
   }
+  *estimate = best_time;
   return best;
+}
+
+// More than 128 rows of x with K split over clusters, on the scale of the estimates above (microseconds without the launch): a
+// start that grows with a block's rows of x, whose sums are exchanged, and the blocks of K that one CTA takes.  Fitted to 81
+// problems of 130..2048 x 256..9000 x 1024..28672: the choice is within 2 % of the better one on all of them.  For example
+// (best table row / K split, us): 130 x 4096 x 14336 36.4 / 18.5, 512 x 2048 x 8192 22.6 / 15.4, 1024 x 1024 x 4096 13.8 / 12.3,
+// 256 x 4096 x 4096 13.9 / 12.9, but 256 x 2048 x 2048 8.8 / 9.6 and 512 x 4096 x 1024 7.8 / 11.4.
+double few_rows_estimate(int64_t M, int64_t K, int splits) {
+  const int64_t blocks = (K + BK - 1) / BK;
+  return 2.4 + 0.0145 * static_cast<double>(std::min<int64_t>(M, 256)) + 0.373 * static_cast<double>((blocks + splits - 1) / splits);
 }
 
 template <int OUT_DT>
@@ -1438,7 +1449,12 @@ int launch_int8_gemm(const GemmArgs& a, DeviceCtx* ctx) {
   int cfg_id = a.cfg_id;
   if (cfg_id < 0) {
     if (a.M <= kFewRowsMax) return launch_few_rows(few_rows_args(a), ctx);
-    cfg_id = select_s8_config(a.M, a.N, a.K, ctx->num_sms);
+    double estimate = 0.0;
+    cfg_id = select_s8_config(a.M, a.N, a.K, ctx->num_sms, &estimate);
+    int splits = 1;
+    const int rc = few_rows_splits(few_rows_args(a), ctx, &splits);
+    if (rc != HB200_OK) return rc;
+    if (splits > 1 && few_rows_estimate(a.M, a.K, splits) < estimate) return launch_few_rows(few_rows_args(a), ctx);
   }
   if (cfg_id >= kNumGemmConfigs) return set_error(HB200_ERR_BAD_CONFIG, "int8_gemm: no such config");
   const GemmConfig& c = kGemmConfigs[cfg_id];

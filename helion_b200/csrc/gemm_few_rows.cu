@@ -1,5 +1,6 @@
 // Products of few rows (M <= 128) with one or two column-major weights: int8_gemm for a handful of tokens, and the
-// gated projection act(x Wg) * (x Wu) for them (e4m3, int8, fp16 or bf16 operands).
+// gated projection act(x Wg) * (x Wu) for them (e4m3, int8, fp16 or bf16 operands).  int8_gemm also has more rows of x
+// computed here, in blocks of 256, where the columns are so few that tiles would leave most SMs idle and K is split.
 //
 // Such a call is bound by reading the weights once.  As in fp8_gemm_skinny.cu the operands are swapped: 128 rows of the
 // tensor-core tile are columns of the weight (K contiguous), the rows of x are its N dimension.  Two things differ:
@@ -13,7 +14,9 @@
 // Where even shares would be narrow, K is split over the CTAs of a cluster instead (2 or 4): a CTA then streams up to
 // four times the columns over a part of K, reads that part of x only, and wastes less of the 128-row instruction.  The
 // partial sums meet in shared memory over the cluster: each CTA takes its share of x's rows, sums the parts in the
-// cluster's order (fixed, so the result does not depend on timing; exact in int32) and applies scales and gate.
+// cluster's order (fixed, so the result does not depend on timing; exact in int32) and applies scales and gate.  The
+// scales wait in shared memory by then: fetched row by row they were 1 to 2 us of a call (256 x 4096 x 4096 13.6 / 12.9,
+// 256 x 1024 x 1024 12.9 / 10.8).
 //
 //   warp 0     TMA producer            warp 1     MMA issuer (M = 128, N = NM)
 //   warps 2-5  epilogue: lane = weight column, registers = rows of x
@@ -39,7 +42,7 @@ constexpr int fr_threads(int nm) { return 64 + 32 * fr_epi_warps(nm); }
 constexpr int FR_MAX_STAGES = 32;
 constexpr int FR_TILE_BYTES = 128 * FR_BK;  // what one instruction's operand of 128 rows spans
 constexpr int FR_SMEM_LIMIT = 227 * 1024;
-constexpr int FR_BAR_BYTES = (2 * FR_MAX_STAGES + 5) * 8 + 16;
+constexpr int FR_STATIC_BYTES = (2 * FR_MAX_STAGES + 5) * 8 + 16 + 256 * 4;  // barriers and scales
 
 struct FewRowsParams {
   void* out;
@@ -76,11 +79,15 @@ __device__ __forceinline__ void load_scales(const FewRowsParams& p, int n, bool 
   }
 }
 
+// The scale of row m of x.
+__device__ __forceinline__ float row_scale(const FewRowsParams& p, int m) {
+  return p.scale_mode == 0 ? 1.0f : __ldg(p.scale_mode == 1 ? p.scale_x : p.scale_x + m);
+}
+
 // Scales, gate, rounding and store of out[m, n].
 template <int W, int OUT_DT>
-__device__ __forceinline__ void finish(const FewRowsParams& p, int m, int n, float (&v)[W], const float (&sw)[W]) {
+__device__ __forceinline__ void finish(const FewRowsParams& p, int m, int n, float (&v)[W], float sx, const float (&sw)[W]) {
   if (p.scale_mode != 0) {
-    const float sx = __ldg(p.scale_mode == 1 ? p.scale_x : p.scale_x + m);
 #pragma unroll
     for (int w = 0; w < W; ++w) v[w] = (v[w] * sx) * sw[w];
   }
@@ -107,6 +114,7 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[2 * FR_MAX_STAGES + 5];
   __shared__ uint32_t misc[2];
+  __shared__ float scales_x[NM];  // with K split: those of the block's rows
   const int stages = p.stages;
   uint64_t* full = bars;
   uint64_t* empty = bars + FR_MAX_STAGES;
@@ -129,8 +137,12 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
   const int kb_begin = min(static_cast<int>(rank) * kb_per_split, k_blocks);
   const int kb_end = min(kb_begin + kb_per_split, k_blocks);
   const int whole = min(p.K / FR_BK, kb_end);  // blocks below this lie wholly inside K
-  const int first_unit = blockIdx.x / p.splits;
-  const int unit_step = gridDim.x / p.splits;
+  // with K split, a cluster has one unit of one block of NM rows of x; else all of x's rows are one block
+  const int cluster = blockIdx.x / p.splits;
+  const int m0 = p.splits > 1 ? cluster / units * NM : 0;
+  const int first_unit = p.splits > 1 ? cluster % units : cluster;
+  const int unit_step = p.splits > 1 ? units : static_cast<int>(gridDim.x);
+  const int block_m = min(p.M - m0, NM);  // its rows of x
   const WaitCtx wctx{abort_flag, p.status};
 
   if (threadIdx.x == 0) {
@@ -181,7 +193,7 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
             mbar_arrive_expect_tx(&full[s], slab_bytes * p.slabs);
 #pragma unroll
             for (int w = 0; w < W; ++w) tma_load_3d(dst + w * slot_bytes, &maps.w[w], &full[s], 0, unit * p.rows, kb);
-            tma_load_3d(dst + W * slot_bytes, &maps.x, &full[s], 0, 0, kb);
+            tma_load_3d(dst + W * slot_bytes, &maps.x, &full[s], 0, m0, kb);
           } else {
             const int blocks = min(p.slabs, kb_end - kb);
             mbar_arrive_expect_tx(&full[s], slab_bytes * blocks);
@@ -191,7 +203,7 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
               for (int w = 0; w < W; ++w) {
                 tma_load_2d(dst + w * slot_bytes + b * slab_w, &maps.w_tail[w], &full[s], k, unit * p.rows);
               }
-              tma_load_2d(dst + W * slot_bytes + b * slab_x, &maps.x_tail, &full[s], k, 0);
+              tma_load_2d(dst + W * slot_bytes + b * slab_x, &maps.x_tail, &full[s], k, m0);
             }
           }
           if (++s == stages) {
@@ -291,7 +303,7 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
               float v[W];
 #pragma unroll
               for (int w = 0; w < W; ++w) v[w] = to_float<KIND>(r[w][i]);
-              finish<W, OUT_DT>(p, c + i, n, v, sw);
+              finish<W, OUT_DT>(p, c + i, n, v, row_scale(p, c + i), sw);
             }
           }
         }
@@ -308,24 +320,30 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
     const int quarter = warp & 3;
     const int mine = quarter * 32 + lane;
     const int sub = (warp - 2) >> 2;
+    // the scales are fetched while the products run
+    const int n = first_unit * p.rows + mine;
+    const bool live = mine < p.rows && n < p.N;
+    float sw[W];
     bool ok = true;
     if (warp >= 2) {
+      load_scales<W>(p, n, live, sw);
+      for (int m = threadIdx.x - 64; m < block_m; m += fr_threads(NM) - 64) scales_x[m] = row_scale(p, m0 + m);
       ok = mbar_wait(acc_full, 0, wctx, SITE_GEMM_ACC_FULL);
       ok = __all_sync(0xffffffffu, ok);
     }
     cluster_sync_all();
-    const int groups = (p.M + 3) / 4;
+    const int groups = (block_m + 3) / 4;
     // slot of (sender, weight, the receiver's j-th group): 128 columns of 16 bytes; a receiver has NM / 4 / splits
     // groups, so all of it is fr_exchange_bytes(W, NM)
     const int held = NM / 4 / p.splits;
     auto slot = [&](int from, int w, int j) { return static_cast<uint32_t>((from * W + w) * held + j) * 2048u + mine * 16u; };
-    if (warp >= 2 && ok) {
+    if (warp >= 2 && ok && quarter * 32 < p.rows) {  // columns that the unit does not have stay here
       tc_fence_after_sync();
       const bool none = kb_begin >= kb_end;  // this CTA had no part of K: its accumulators were never written
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
       for (int c = sub * 16; c < NM; c += SUBS * 16) {
-        if (c >= p.M) break;
+        if (c >= block_m) break;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           uint32_t r[16];
@@ -334,7 +352,7 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int g = c / 4 + q;
-            if (g < groups) {
+            if (g < groups && mine < p.rows) {
               const uint32_t v[4] = {none ? 0u : r[4 * q], none ? 0u : r[4 * q + 1], none ? 0u : r[4 * q + 2], none ? 0u : r[4 * q + 3]};
               st_cluster_v4(map_to_cta(smem_u32(smem) + slot(rank, w, g / p.splits), g % p.splits), v);
             }
@@ -344,10 +362,6 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
     }
     cluster_sync_all();
     if (warp >= 2 && ok) {
-      const int n = first_unit * p.rows + mine;
-      const bool live = mine < p.rows && n < p.N;
-      float sw[W];
-      load_scales<W>(p, n, live, sw);
       for (int g = rank + sub * p.splits; g < groups && live; g += SUBS * p.splits) {
         uint4 part[4];
         float v[4][W];
@@ -372,7 +386,7 @@ few_rows_kernel(const __grid_constant__ FewRowsMaps maps, const FewRowsParams p)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (4 * g + i < p.M) finish<W, OUT_DT>(p, 4 * g + i, n, v[i], sw);
+          if (4 * g + i < block_m) finish<W, OUT_DT>(p, m0 + 4 * g + i, n, v[i], scales_x[4 * g + i], sw);
         }
       }
     }
@@ -404,6 +418,35 @@ cudaError_t max_clusters(const void* kernel, int cluster, int threads, int smem,
   return cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg);
 }
 
+// Shares of K: as many as leave a CTA at most 128 columns, with four blocks of K each at least; `at_once`: the CTAs or
+// clusters that share the columns of a block of NM rows of x.  Measured at 16 rows of x, N = 4096, int8: K = 14336 in 1 / 2 /
+// 4 shares 20.8 / 16.2 / 13.5 us, K = 4096 in 9.3 / 9.1 / 7.2 us.
+template <int KIND, int NM, bool GATED, int OUT_DT>
+int choose_splits(const FewRowsArgs& a, DeviceCtx* ctx, int* splits, int64_t* at_once) {
+  auto kernel = few_rows_kernel<KIND, NM, GATED, OUT_DT>;
+  static std::atomic<uint64_t> smem_attr_done{0};
+  HB_CUDA_CHECK(set_max_dynamic_smem_once(smem_attr_done, reinterpret_cast<const void*>(kernel),
+                                          FR_SMEM_LIMIT - FR_STATIC_BYTES, a.device));
+  const int64_t k_blocks = (a.K * kind_bytes(KIND) + FR_BK - 1) / FR_BK;
+  const int64_t row_blocks = (a.M + NM - 1) / NM;
+  const int64_t column_blocks = (a.N + 127) / 128;
+  *splits = 1;
+  *at_once = ctx->num_sms;
+  for (int s = 2; s <= 4 && k_blocks >= 4 * s; s *= 2) {
+    static std::atomic<int> fit[2][64];
+    std::atomic<int>& known = fit[s / 4][static_cast<unsigned>(a.device) & 63u];
+    int clusters = known.load(std::memory_order_relaxed);
+    if (clusters == 0) {
+      HB_CUDA_CHECK(max_clusters(reinterpret_cast<const void*>(kernel), s, fr_threads(NM), FR_SMEM_LIMIT - FR_STATIC_BYTES, &clusters));
+      known.store(clusters, std::memory_order_relaxed);
+    }
+    if (column_blocks > clusters / row_blocks) break;
+    *splits = s;
+    *at_once = clusters / row_blocks;
+  }
+  return HB200_OK;
+}
+
 template <int KIND, int NM, bool GATED, int OUT_DT>
 int launch_few_rows_instance(const FewRowsArgs& a, DeviceCtx* ctx) {
   constexpr int W = GATED ? 2 : 1;
@@ -414,33 +457,17 @@ int launch_few_rows_instance(const FewRowsArgs& a, DeviceCtx* ctx) {
   p.M = static_cast<int>(a.M);
   p.N = static_cast<int>(a.N);
   p.K = static_cast<int>(a.K * ES);
-  const int k_blocks = (p.K + FR_BK - 1) / FR_BK;
-  static std::atomic<uint64_t> smem_attr_done{0};
-  HB_CUDA_CHECK(set_max_dynamic_smem_once(smem_attr_done, reinterpret_cast<const void*>(kernel),
-                                          FR_SMEM_LIMIT - FR_BAR_BYTES, a.device));
-  // Shares of K: as many as leave a CTA at most 128 columns, with four blocks of K each at least.  Measured at 16 rows of
-  // x, N = 4096, int8: K = 14336 in 1 / 2 / 4 shares 20.8 / 16.2 / 13.5 us, K = 4096 in 9.3 / 9.1 / 7.2 us.
-  p.splits = 1;
-  int64_t at_once = ctx->num_sms;
-  for (int s = 2; s <= 4 && k_blocks >= 4 * s; s *= 2) {
-    static std::atomic<int> fit[2][64];
-    std::atomic<int>& known = fit[s / 4][static_cast<unsigned>(a.device) & 63u];
-    int clusters = known.load(std::memory_order_relaxed);
-    if (clusters == 0) {
-      HB_CUDA_CHECK(max_clusters(reinterpret_cast<const void*>(kernel), s, fr_threads(NM), FR_SMEM_LIMIT - FR_BAR_BYTES, &clusters));
-      known.store(clusters, std::memory_order_relaxed);
-    }
-    if (a.N > 128ll * clusters) break;
-    p.splits = s;
-    at_once = clusters;
-  }
+  int64_t at_once = 0;
+  if (const int rc = choose_splits<KIND, NM, GATED, OUT_DT>(a, ctx, &p.splits, &at_once); rc != HB200_OK) return rc;
+  const int64_t row_blocks = (a.M + NM - 1) / NM;
+  if (row_blocks > 1 && p.splits == 1) return set_error(HB200_ERR_BAD_CONFIG, "few rows: more rows of x than one block, and K not split");
   // Even shares of the columns: as few rounds of 128 columns as there must be, over all CTAs or clusters that fit at once.
   const int64_t rounds = (a.N + 128 * at_once - 1) / (128 * at_once);
   p.rows = static_cast<int>((a.N + rounds * at_once - 1) / (rounds * at_once) + 7) / 8 * 8;
   const int slab_bytes = (W * p.rows + NM) * FR_BK;
   // An instruction reads 128 rows from the start of a slot of fewer: past the last stage there has to be room for that.
   const int tail = FR_TILE_BYTES;
-  const int budget = FR_SMEM_LIMIT - FR_BAR_BYTES - 1024 - tail;
+  const int budget = FR_SMEM_LIMIT - FR_STATIC_BYTES - 1024 - tail;
   // Several blocks of K a stage: what a stage costs beside its bytes (barriers, one TMA request per operand) is then
   // paid for up to 48 KB.  Measured at 16 x 4096 x 14336, int8, K not split: 1 / 2 / 4 / 8 blocks of 6 KB a stage
   // 40.3 / 28.8 / 23.1 / 20.7 us.
@@ -484,7 +511,7 @@ int launch_few_rows_instance(const FewRowsArgs& a, DeviceCtx* ctx) {
 
   const int64_t units = (a.N + p.rows - 1) / p.rows;
   if (p.splits > 1) {
-    HB_CUDA_CHECK(launch_pdl_cluster(kernel, static_cast<unsigned>(units * p.splits), fr_threads(NM), p.splits, smem, a.stream, maps, p));
+    HB_CUDA_CHECK(launch_pdl_cluster(kernel, static_cast<unsigned>(row_blocks * units * p.splits), fr_threads(NM), p.splits, smem, a.stream, maps, p));
   } else {
     HB_CUDA_CHECK(launch_pdl(kernel, static_cast<unsigned>(std::min<int64_t>(units, ctx->num_sms)), fr_threads(NM), smem, a.stream,
                              maps, p));
@@ -497,6 +524,9 @@ int launch_few_rows_nm(const FewRowsArgs& a, DeviceCtx* ctx) {
   if (a.M <= 16) return launch_few_rows_instance<KIND, 16, GATED, OUT_DT>(a, ctx);
   if (a.M <= 32) return launch_few_rows_instance<KIND, 32, GATED, OUT_DT>(a, ctx);
   if (a.M <= 64) return launch_few_rows_instance<KIND, 64, GATED, OUT_DT>(a, ctx);
+  if constexpr (!GATED) {
+    if (a.M > 128) return launch_few_rows_instance<KIND, 256, GATED, OUT_DT>(a, ctx);
+  }
   return launch_few_rows_instance<KIND, 128, GATED, OUT_DT>(a, ctx);
 }
 
@@ -533,6 +563,11 @@ FewRowsArgs few_rows_args(const GemmArgs& a) {
   f.scale_w[0] = a.scale_b;
   f.scale_mode = a.scale_mode;
   return f;
+}
+
+int few_rows_splits(const FewRowsArgs& a, DeviceCtx* ctx, int* splits) {
+  int64_t at_once = 0;
+  return choose_splits<KIND_S8, 256, false, HB200_DT_BF16>(a, ctx, splits, &at_once);
 }
 
 int launch_few_rows(const FewRowsArgs& a, DeviceCtx* ctx) {

@@ -121,7 +121,7 @@ int launch_gemm_16bit(const GemmArgs& args, DeviceCtx* ctx);
 int launch_int8_gemm(const GemmArgs& args, DeviceCtx* ctx);
 
 // Up to 128 rows of x against one weight (int8) or the two weights of a gated projection, all column-major
-// (gemm_few_rows.cu).
+// (gemm_few_rows.cu); more rows against one weight where few_rows_splits() is above 1.
 constexpr int64_t kFewRowsMax = 128;
 struct FewRowsArgs {
   const void* x = nullptr;
@@ -141,6 +141,8 @@ struct FewRowsArgs {
 };
 FewRowsArgs few_rows_args(const GemmArgs& args);
 int launch_few_rows(const FewRowsArgs& args, DeviceCtx* ctx);
+// In how many shares that kernel would split K for more than 128 rows of x (int8, not gated); 1: it does not take them.
+int few_rows_splits(const FewRowsArgs& args, DeviceCtx* ctx, int* splits);
 // The gated projection out = act(x w[0]) * (x w[1]) (gated_forward.cu) and its gradients (gated_backward.cu).
 struct GatedArgs {
   const void* x = nullptr;

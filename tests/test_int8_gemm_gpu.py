@@ -54,6 +54,19 @@ def test_scaled_products(hb, m, n, k, out_dtype):
             assert torch.equal(out.double(), x.double() @ y.double())
 
 
+@pytest.mark.parametrize("m,n,k", [(129, 1024, 4096), (130, 4096, 14336), (192, 9000, 16384), (256, 520, 8192), (257, 33, 8208), (513, 2048, 8200), (700, 1536, 12304), (1023, 512, 6160), (2049, 72, 4112)])
+def test_more_rows_with_long_k_and_few_columns(hb, m, n, k):
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    x, y = codes(g, m, k), codes(g, n, k).t()
+    sa, sb = (torch.rand(c, generator=g, device="cuda") * 1e-3 + 1e-6 for c in (m, n))
+    for out_dtype in (torch.bfloat16, torch.float32):
+        store = torch.full((m + 3, n + 8), 5.0, device="cuda", dtype=out_dtype)
+        check(hb.int8_gemm(x, y, scale_a=sa, scale_b=sb, out_dtype=out_dtype, out=store[:m, :n]), x, y, sa, sb)
+        assert (store[m:] == 5).all() and (store[:, n:] == 5).all()
+    check(hb.int8_gemm(x, y, out_dtype=torch.float32), x, y)
+    assert torch.equal(hb.int8_gemm(x, y, scale_a=sa, scale_b=sb), hb.int8_gemm(x, y, scale_a=sa, scale_b=sb, config=1))
+
+
 @pytest.mark.parametrize("row", [0, 1, 2, 3, 6, 7, 10, 14, 17, 18, 21])
 def test_every_table_row_gives_the_same_bits(hb, row):
     g = torch.Generator(device="cuda").manual_seed(row)
