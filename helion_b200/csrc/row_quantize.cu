@@ -227,14 +227,14 @@ __device__ __forceinline__ void set_pair(float (&v)[8], int i, uint64_t pair) {
   v[2 * i + 1] = __uint_as_float(b);
 }
 
-template <int TIER, int MODE>
+template <int TIER>
 __device__ __forceinline__ void store_codes(uint8_t* row, int lo, int N, const float (&t)[8], float2 f, bool int8) {
   float v[8];
   const uint64_t hi = pack2f(f.x, f.x), lo2 = pack2f(f.y, f.y);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint64_t t2 = pack2f(t[2 * i], t[2 * i + 1]);
-    set_pair(v, i, MODE == 0 ? fmul2(t2, hi) : ffma2(t2, hi, fmul2(t2, lo2)));
+    set_pair(v, i, ffma2(t2, hi, fmul2(t2, lo2)));
   }
   const uint32_t a = code4(v[0], v[1], v[2], v[3], int8);
   const uint32_t b = code4(v[4], v[5], v[6], v[7], int8);
@@ -248,9 +248,10 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int lo, int N, const f
   }
 }
 
-// One row's factor Q / max for the codes, as a sum of two floats, and its scale.  Products of few bits often lie exactly between
-// two codes; the factor's own rounding would decide these ties by chance (8192 x 4096 bf16 with residual: 104 codes of 33.6
-// million differed from the exact ones, with two floats none).  Without the norm one float was as exact (none of 58.7 million).
+// One row's factor Q / max for the codes, as a sum of two floats, and its scale.  Values of few bits often lie exactly between
+// two codes (max / 2 does for int8); the factor's own rounding would decide these ties by chance: with one float 2.734375 in a
+// row with the maximum 3.0625 is 400.00003 instead of 400 and gets the code 416 instead of 384.  With two the product is within
+// 2^-46 before its rounding to fp32, and every code of 16-bit values is that of the exact quotient.
 template <int MODE>
 __device__ __forceinline__ float2 row_factor(const RowQuantArgs& a, float sum, uint32_t top, float& scale) {
   const float Q = a.int8 ? 127.0f : 448.0f;
@@ -267,7 +268,7 @@ __device__ __forceinline__ float2 row_factor(const RowQuantArgs& a, float sum, u
     scale = kTiny;
     f = 0.0f;
   }
-  return make_float2(f, MODE != 0 && f > 0.0f ? fmaf(-f, amax, Q) * (f / Q) : 0.0f);
+  return make_float2(f, f > 0.0f ? fmaf(-f, amax, Q) * (f * (a.int8 ? 1.0f / 127.0f : 1.0f / 448.0f)) : 0.0f);
 }
 
 // t += r, two values an instruction (the kernels issue close to what an SM can where rows come fast).
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int g = threadIdx.x + v * blockDim.x;
-      if (g < groups) store_codes<TIER, MODE>(codes, first + g * 8, N, t[v], f, a.int8);
+      if (g < groups) store_codes<TIER>(codes, first + g * 8, N, t[v], f, a.int8);
     }
   } else {
     for (int g = threadIdx.x; g < groups; g += blockDim.x) {
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
       uint32_t t2 = 0;
       load(g, t[0], rv[0]);
       take(g, t[0], rv[0], s2, t2, true);
-      store_codes<TIER, MODE>(codes, first + g * 8, N, t[0], f, a.int8);
+      store_codes<TIER>(codes, first + g * 8, N, t[0], f, a.int8);
     }
   }
 }
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(VPT == 2 ? 1024 : 512) row_ring_kernel(RowQuan
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int g = threadIdx.x + v * blockDim.x;
-      if (g < groups) store_codes<ROW_ALIGNED, MODE>(codes, g * 8, 0, t[v], f, a.int8);
+      if (g < groups) store_codes<ROW_ALIGNED>(codes, g * 8, 0, t[v], f, a.int8);
     }
     turn ^= 1u;
     if (++s == ring.stages) {
