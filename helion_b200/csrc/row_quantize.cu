@@ -55,8 +55,10 @@ enum RowTier : int {
 };
 
 constexpr uint32_t kF32AbsMask = 0x7fffffffu;
-// Rows whose largest |s w| is below this are rows of zeros (Q / max could overflow).
+// Rows whose largest |y| is below this are rows of zeros (Q / max|y| may overflow).
 constexpr float kZeroRow = 7.888609e-31f;  // 2^-100
+// Behind the norm |s w| may be smaller where |y| is not: such a row's values are multiplied by this before the factor.
+constexpr float kLift = 18446744073709551616.0f;  // 2^64: the smallest positive |s w|, 2^-149, becomes 2^-85
 
 template <int SRC_DT>
 struct Src;
@@ -252,23 +254,31 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int lo, int N, const f
 // two codes (max / 2 does for int8); the factor's own rounding would decide these ties by chance: with one float 2.734375 in a
 // row with the maximum 3.0625 is 400.00003 instead of 400 and gets the code 416 instead of 384.  With two the product is within
 // 2^-46 before its rounding to fp32, and every code of 16-bit values is that of the exact quotient.
+// `lift`: the values need kLift first.
 template <int MODE>
-__device__ __forceinline__ float2 row_factor(const RowQuantArgs& a, float sum, uint32_t top, float& scale) {
+__device__ __forceinline__ float2 row_factor(const RowQuantArgs& a, float sum, uint32_t top, float& scale, bool& lift) {
   const float Q = a.int8 ? 127.0f : 448.0f;
-  constexpr float kTiny = 1.17549435e-38f;
-  const float amax = __uint_as_float(top);
-  float rstd = 1.0f;
+  float amax = __uint_as_float(top);
+  float y_max = amax;
+  lift = false;
   if constexpr (MODE != 0) {
     // a sum of squares beyond fp32 (or one that holds an infinity or a NaN) makes the row's scale NaN
-    rstd = sum <= 3.402823466e38f ? 1.0f / sqrtf(sum * a.inv_n + a.eps) : __uint_as_float(0x7fc00000u);
+    y_max *= sum <= 3.402823466e38f ? 1.0f / sqrtf(sum * a.inv_n + a.eps) : __uint_as_float(0x7fc00000u);
+    lift = amax < kZeroRow;
+    if (lift) amax *= kLift;
   }
-  scale = amax * rstd / Q;
+  scale = y_max / Q;
   float f = Q / amax;
-  if (amax < kZeroRow || scale < kTiny) {
-    scale = kTiny;
+  if (y_max < kZeroRow) {
+    scale = 1.17549435e-38f;
     f = 0.0f;
   }
   return make_float2(f, f > 0.0f ? fmaf(-f, amax, Q) * (f * (a.int8 ? 1.0f / 127.0f : 1.0f / 448.0f)) : 0.0f);
+}
+
+__device__ __forceinline__ void lift_group(float (&t)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] *= kLift;
 }
 
 // t += r, two values an instruction (the kernels issue close to what an SM can where rows come fast).
@@ -387,10 +397,15 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
     warp_reduce<MODE>(sum, top);
   }
   float scale;
-  const float2 f = row_factor<MODE>(a, sum, top, scale);
+  bool lift;
+  const float2 f = row_factor<MODE>(a, sum, top, scale, lift);
   if (threadIdx.x == 0) a.scales[row] = scale;
 
   if constexpr (VPT > 0) {
+    if (MODE != 0 && lift) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) lift_group(t[v]);
+    }
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int g = threadIdx.x + v * blockDim.x;
@@ -402,6 +417,7 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
       uint32_t t2 = 0;
       load(g, t[0], rv[0]);
       take(g, t[0], rv[0], s2, t2, true);
+      if (MODE != 0 && lift) lift_group(t[0]);
       store_codes<TIER>(codes, first + g * 8, N, t[0], f, a.int8);
     }
   }
@@ -507,8 +523,13 @@ __global__ void __launch_bounds__(VPT == 2 ? 1024 : 512) row_ring_kernel(RowQuan
     top = lane < warps ? red_max[turn][lane] : 0u;
     warp_reduce<MODE>(sum, top);
     float scale;
-    const float2 f = row_factor<MODE>(a, sum, top, scale);
+    bool lift;
+    const float2 f = row_factor<MODE>(a, sum, top, scale, lift);
     if (threadIdx.x == 0) a.scales[row] = scale;
+    if (MODE != 0 && lift) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) lift_group(t[v]);
+    }
     uint8_t* codes = reinterpret_cast<uint8_t*>(a.codes) + row * a.codes_rs;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {

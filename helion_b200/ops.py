@@ -519,8 +519,9 @@ def rms_norm_quantize(
     residual of the next layer.  The norm takes the fp32 sum before that rounding.  ``x`` and ``residual`` share one
     dtype (fp16, bf16, fp32); ``weight [N]`` has it too or is fp32.  ``residual_out`` may be ``x`` or ``residual``
     itself (an update in place); ``eps`` is a positive normal fp32 number; ``out``, ``scale_out`` and ``residual_out``
-    are contiguous and overlap nothing else.  A row whose sum of squares is not finite in fp32 gets a NaN scale.  The
-    results have no gradient.
+    are contiguous and overlap nothing else.  A row of zeros (``max|y| < 2**-100``) gets zero codes and the smallest normal
+    scale; a row whose sum of squares is not finite in fp32 gets a NaN scale, one whose ``max|s * weight|`` alone is not
+    an infinite one.  The results have no gradient.
     """
     source, target = _check_row_input(x, out_dtype, "rms_norm_quantize")
     shape, dtype = x.shape, x.dtype

@@ -268,8 +268,8 @@ HB200_API int hb200_quantize_rows(const void* x, void* codes, float* scales, int
  *   residual: NULL (s = x; residual_out must then be NULL too), else [M,N] of src_dtype;
  *   residual_out: [M,N] of src_dtype; may be x or residual itself (same pointer and stride), no other overlap;
  *   weight: N values, weight_dtype = src_dtype or FP32.  eps: a positive normal fp32 number.
- * A row whose max|s * weight| is below 2^-100, or whose scale would be below FLT_MIN, gets codes of zero and the
- * scale FLT_MIN; a sum of squares that is not finite in fp32 makes the row's scale NaN. */
+ * A row whose max|y| is below 2^-100 gets codes of zero and the scale FLT_MIN; a sum of squares that is not finite in
+ * fp32 makes the row's scale NaN, a finite one with max|s * weight| beyond fp32 makes it infinite. */
 HB200_API int hb200_rms_norm_quantize(const void* x, const void* residual, const void* weight, void* codes, float* scales,
                                       void* residual_out, int64_t M, int64_t N, int64_t x_rs, int64_t residual_rs,
                                       int64_t codes_rs, int64_t residual_out_rs, int src_dtype, int weight_dtype,
