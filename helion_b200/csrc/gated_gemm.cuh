@@ -82,12 +82,12 @@ __device__ __forceinline__ void gated_scale(uint32_t (&r)[32], const GatedParams
   scales_only_chunk(r, sc, row, p.M, col, p.N);
 }
 
-template <int ACT>
+template <int ACT, bool FINE>
 __device__ __forceinline__ void gate_chunk(uint32_t (&g)[32], const uint32_t (&u)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     float a, d;
-    activate<ACT, false>(__uint_as_float(g[i]), a, d);
+    activate<ACT, false, FINE>(__uint_as_float(g[i]), a, d);
     g[i] = __float_as_uint(a * __uint_as_float(u[i]));
   }
 }
@@ -99,7 +99,7 @@ __device__ __forceinline__ void gate_chunk_train(uint32_t (&g)[32], uint32_t (&u
   for (int i = 0; i < 32; ++i) {
     float a, d;
     const float uf = __uint_as_float(u[i]);
-    activate<ACT, true>(__uint_as_float(g[i]), a, d);
+    activate<ACT, true, false>(__uint_as_float(g[i]), a, d);
     h[i] = __float_as_uint(a * uf);
     g[i] = __float_as_uint(a);
     u[i] = __float_as_uint(uf * d);
@@ -326,9 +326,10 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
           gated_scale<KIND>(r, p, 0, row0 + lane, col);
           gated_scale<KIND>(u, p, 1, row0 + lane, col);
           if constexpr (MODE == MODE_GATED) {
-            if (p.act == ACT_SILU) gate_chunk<ACT_SILU>(r, u);
-            else if (p.act == ACT_GELU) gate_chunk<ACT_GELU>(r, u);
-            else gate_chunk<ACT_GELU_TANH>(r, u);
+            constexpr bool FINE = OUT_DT == HB200_DT_FP32;
+            if (p.act == ACT_SILU) gate_chunk<ACT_SILU, FINE>(r, u);
+            else if (p.act == ACT_GELU) gate_chunk<ACT_GELU, FINE>(r, u);
+            else gate_chunk<ACT_GELU_TANH, FINE>(r, u);
             StagedStore<OUT_DT>::store(r, stage, chunk_count, lane, &maps.out[0], col, row0, inside);
           } else {
             uint32_t h[32];

@@ -92,7 +92,7 @@ __device__ __forceinline__ void finish(const FewRowsParams& p, int m, int n, flo
     for (int w = 0; w < W; ++w) v[w] = (v[w] * sx) * sw[w];
   }
   float o = v[0];
-  if constexpr (W == 2) o = activate_by(p.act, v[0]) * v[1];
+  if constexpr (W == 2) o = activate_by<OUT_DT == HB200_DT_FP32>(p.act, v[0]) * v[1];
   const int64_t at = static_cast<int64_t>(m) * p.ldc + n;
   if constexpr (OUT_DT == HB200_DT_FP32) {
     reinterpret_cast<float*>(p.out)[at] = o;
