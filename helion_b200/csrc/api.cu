@@ -658,7 +658,8 @@ static size_t gated_products_bytes(int64_t M, int64_t F) { return 4 * static_cas
 
 size_t hb200_gated_gemm_backward_workspace_bytes(int64_t M, int64_t F, int64_t K) {
   if (M < 1 || F < 1 || K < 1) return 0;
-  return gated_products_bytes(M, F) + gated_grad_partial_bytes(M, F, K, query_num_sms());
+  const int sms = query_num_sms();
+  return gated_products_bytes(M, F) + gated_grad_range_bytes(sms) + gated_grad_partial_bytes(M, F, K, sms);
 }
 
 int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const float* saved_p,
@@ -694,8 +695,9 @@ int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate,
   }
   DeviceCtx* ctx = get_device_ctx(device);
   if (ctx == nullptr) return ctx_error_code(device);
-  const size_t partials_at = gated_products_bytes(M, F);
-  if (dx != nullptr && workspace_bytes < partials_at + gated_grad_partial_bytes(M, F, K, ctx->num_sms)) {
+  const size_t range_at = gated_products_bytes(M, F);
+  const size_t partials_at = range_at + gated_grad_range_bytes(ctx->num_sms);
+  if (workspace_bytes < partials_at + (dx != nullptr ? gated_grad_partial_bytes(M, F, K, ctx->num_sms) : 0)) {
     return set_error(HB200_ERR_WORKSPACE, "gated_gemm_backward: needs a 16-byte aligned workspace of "
                                           "hb200_gated_gemm_backward_workspace_bytes(M, F, K)");
   }
@@ -710,6 +712,7 @@ int hb200_gated_gemm_backward(const void* dh, const void* x, const void* w_gate,
   a.dw[0] = dw_gate;
   a.dw[1] = dw_up;
   a.dgu = workspace;
+  a.range = reinterpret_cast<float*>(static_cast<char*>(workspace) + range_at);
   a.partials = static_cast<char*>(workspace) + partials_at;
   a.M = M;
   a.F = F;

@@ -70,7 +70,7 @@ struct GatedParams {
   int group_m;
   int act;
   uint32_t* status;
-  const float *scale_x, *scale_w[2];
+  const float *scale_x, *scale_w[2];  // gradients: scale_x is the factor of all results of fp16 operands
   int scale_mode;
 };
 
@@ -302,6 +302,7 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
     uint8_t* stage = smem + L::EPI_OFFSET + (warp - 2) * L::WARP_EPI_BYTES;
     uint32_t chunk_count = 0;
     uint32_t tile_iter = 0;
+    const float factor = !GATED && KIND == KIND_F16 ? *p.scale_x : 1.0f;  // written by the kernel before this one
     for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++tile_iter) {
       const int layer = LAYERS ? tile / one : 0;
       const TileCoord tc = tile_coord(tile - layer * one, m_tiles, n_tiles, p.group_m);
@@ -344,6 +345,10 @@ gated_pair_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
           }
         } else {
           tmem_wait_ld();
+          if constexpr (KIND == KIND_F16) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * factor);
+          }
           if constexpr (MODE == MODE_SUM_SPLIT) {
             constexpr int KEEP = StagedStore<OUT_DT>::NBUF - 1;
             StagedStore<OUT_DT>::template store<KEEP, true>(r, stage, chunk_count, lane, &maps.out[0], col, row0, inside, nullptr, layer);

@@ -170,6 +170,7 @@ struct GatedGradArgs {
   void* dx = nullptr;                      // null: not wanted
   void* dw[2] = {nullptr, nullptr};        // null: not wanted
   void* dgu = nullptr;                     // workspace: dG and dU, [M,F] each of the operands' type
+  float* range = nullptr;                  // workspace: gated_grad_range_bytes
   void* partials = nullptr;                // workspace: gated_grad_partial_bytes, needed for dx
   int64_t M = 0, F = 0, K = 0;
   int64_t dh_rs = 0, lda = 0, ldb[2] = {0, 0};
@@ -179,6 +180,8 @@ struct GatedGradArgs {
   cudaStream_t stream = nullptr;
 };
 int launch_gated_grad(const GatedGradArgs& args, DeviceCtx* ctx);
+// What the fp16 products keep of their range (a multiple of 128).
+size_t gated_grad_range_bytes(int num_sms);
 // fp32 partial sums of dx where its K loop is split (0: it is not).
 size_t gated_grad_partial_bytes(int64_t M, int64_t F, int64_t K, int num_sms);
 int gemm_num_configs();

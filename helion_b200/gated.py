@@ -145,7 +145,8 @@ def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     fp32 accumulation; the result has the operands' dtype, rounded once.  The weights may be column-major (a transposed
     view of ``[F, K]`` storage) or row-major, both in the same layout (else one is copied).  When a gradient is needed
     the forward pass also keeps two fp32 ``[M,F]`` tensors; the backward pass returns ``x``'s and the weights' gradients
-    in their dtype, and is not differentiable itself.  Both passes can be captured into a CUDA graph, unless an eager
+    in their dtype, and is not differentiable itself.  It rounds ``dh * u * act'(g)`` and ``dh * act(g)`` to the operands'
+    dtype (in fp16 scaled so that their largest value fits) before the products that give the gradients.  Both passes can be captured into a CUDA graph, unless an eager
     graph over the same leaf tensors, made on the default stream, is alive: that is refused.
     """
     if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float16, torch.bfloat16):

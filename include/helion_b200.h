@@ -233,7 +233,8 @@ HB200_API int hb200_gated_gemm(const void* x, const void* w_gate, const void* w_
                                void* stream);
 
 /* Gradients of hb200_gated_gemm with 16-bit operands, from dh [M,F] and what the forward call saved:
- *   dG = dh * saved_p, dU = dh * saved_a (rounded to dtype: operands of the products that follow),
+ *   dG = dh * saved_p, dU = dh * saved_a (rounded to dtype: operands of the products that follow; in FP16 both times
+ *   one power of two, divided out of the results, where the larger of them leaves [2^-6, 65504]),
  *   dx = dG @ w_gate^T + dU @ w_up^T,  dw_gate = x^T @ dG,  dw_up = x^T @ dU;  fp32 accumulation.
  *   dx: [M,K] contiguous, or NULL;  dw_gate, dw_up: [K,F] in the weights' layout without gaps, or both NULL.
  *   workspace: hb200_gated_gemm_backward_workspace_bytes(M, F, K) of device memory, 16-byte aligned, used on `stream` only.
@@ -244,7 +245,7 @@ HB200_API int hb200_gated_gemm_backward(const void* dh, const void* x, const voi
                                         int64_t gate_cs, int64_t up_rs, int64_t up_cs, int dtype, void* workspace,
                                         size_t workspace_bytes, int device, void* stream);
 
-/* Bytes of workspace hb200_gated_gemm_backward needs on the current device: dG and dU, and partial sums of dx where few
+/* Bytes of workspace hb200_gated_gemm_backward needs on the current device: dG and dU, their largest magnitudes, and partial sums of dx where few
  * rows and columns of it leave it to be split along F. */
 HB200_API size_t hb200_gated_gemm_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 
