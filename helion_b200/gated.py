@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _OUT_DT, _empty_matrix, _require_cuda, _round_up, _stream_ptr
+from .ops import _OUT_DT, _changed, _empty_matrix, _require_cuda, _round_up, _stream_ptr
 
 _ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
 
@@ -226,6 +226,7 @@ def gated_gemm(
     m, k = x.shape
     f = w_gate.shape[1]
     scales, mode = _gated_scales(scale_x, scale_gate, scale_up, m, f, dev)
+    given = out
     if out is None:
         out = _empty_matrix(x, m, f, out_dtype)
     elif out.dtype != out_dtype or tuple(out.shape) != (m, f) or out.stride(1) != 1 or out.device != x.device:
@@ -250,4 +251,7 @@ def gated_gemm(
         return out
     x = _rows_ready(x, 16)
     w_gate, w_up = _weights_ready(w_gate, w_up, 16, False)
-    return _launch(x, w_gate, w_up, out, act, dev, "gated_gemm", scales, mode)
+    _launch(x, w_gate, w_up, out, act, dev, "gated_gemm", scales, mode)
+    if given is not None:
+        _changed(given)
+    return out

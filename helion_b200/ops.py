@@ -221,6 +221,7 @@ def int8_gemm(
     mode = _lib.SCALE_NONE
     if scale_a is not None or scale_b is not None:
         scale_a, scale_b, mode = _check_scales(scale_a, scale_b, m, n, x.device, "int8_gemm")
+    given = out
     if out is None:
         out = _empty_matrix(x, m, n, out_dtype)
     elif out.dtype != out_dtype or tuple(out.shape) != (m, n) or out.stride(1) != 1 or out.device != x.device:
@@ -251,6 +252,8 @@ def int8_gemm(
     )
     if code:
         _lib.raise_for(code, "int8_gemm")
+    if given is not None:
+        _changed(given)
     return out
 
 
@@ -451,6 +454,13 @@ def _out_rows(out: Optional[torch.Tensor], like: torch.Tensor, shape, dtype: tor
     return out
 
 
+def _changed(*given: Optional[torch.Tensor]) -> None:
+    """Tells autograd that a kernel wrote the caller's tensors: a graph that saved one of them then refuses its backward pass."""
+    for t in given:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
+
+
 _ROW_SOURCES = {torch.float16: _lib.DT_FP16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_FP32}
 _ROW_CODES = {torch.float8_e4m3fn: _lib.DT_E4M3, torch.int8: _lib.DT_INT8}
 
@@ -498,6 +508,8 @@ def quantize_rows(
     )
     if code:
         _lib.raise_for(code, "quantize_rows")
+    if out is not None or scale_out is not None:
+        _changed(out, scale_out)
     return codes, scales
 
 
@@ -562,6 +574,8 @@ def rms_norm_quantize(
         )
         if code:
             _lib.raise_for(code, "rms_norm_quantize")
+        if out is not None or scale_out is not None or residual_out is not None:
+            _changed(out, scale_out, residual_out)
     return (codes, scales) if residual is None else (codes, scales, summed)
 
 
