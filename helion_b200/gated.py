@@ -66,8 +66,27 @@ def _launch(x, w_gate, w_up, out, act: int, dev: int, what: str, scales=None, mo
     return out
 
 
+class _LivingNodes:
+    """Weak references to backward nodes, for any number of threads: every access to the dictionary is one operation of its
+    own (a WeakSet that is iterated while another thread adds to it raises)."""
+
+    def __init__(self):
+        self._refs = {}
+
+    def add(self, node) -> None:
+        key = id(node)  # not taken by another node before this one's reference has left
+        self._refs[key] = weakref.ref(node, lambda _: self._refs.pop(key, None))
+
+    def snapshot(self) -> list:
+        nodes = (ref() for ref in self._refs.copy().values())
+        return [n for n in nodes if n is not None]
+
+    def __len__(self) -> int:
+        return len(self._refs)
+
+
 # Backward nodes of eager forward passes on the default stream that are still alive (see _refuse_capture).
-_eager_nodes: "weakref.WeakSet" = weakref.WeakSet()
+_eager_nodes = _LivingNodes()
 
 
 class _GatedMatmul(torch.autograd.Function):
@@ -125,7 +144,7 @@ def _refuse_capture(*leaves: torch.Tensor) -> None:
     would be lost in the middle of the backward pass.  So it is refused here, before anything is recorded.
     """
     edges = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t.requires_grad and t.grad_fn is None]
-    seen, todo = set(), list(_eager_nodes)
+    seen, todo = set(), _eager_nodes.snapshot()
     while todo:
         node = todo.pop()
         if any(node is e for e in edges):
@@ -146,8 +165,12 @@ def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     view of ``[F, K]`` storage) or row-major, both in the same layout (else one is copied).  When a gradient is needed
     the forward pass also keeps two fp32 ``[M,F]`` tensors; the backward pass returns ``x``'s and the weights' gradients
     in their dtype, and is not differentiable itself.  It rounds ``dh * u * act'(g)`` and ``dh * act(g)`` to the operands'
-    dtype (in fp16 scaled so that their largest value fits) before the products that give the gradients.  Both passes can be captured into a CUDA graph, unless an eager
-    graph over the same leaf tensors, made on the default stream, is alive: that is refused.
+    dtype (in fp16 scaled so that their largest value fits) before the products that give the gradients.
+
+    Both passes can be captured into a CUDA graph, unless an eager graph over the same leaf tensors, made by this
+    function on the default stream, is alive: a call under capture that needs gradients is refused then.  (Other eager
+    graphs over them, made on the default stream by other operations alone, break a captured backward pass just as
+    they do without this function, and are not seen here.)
     """
     if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"gated_matmul expects three float16 or three bfloat16 tensors, got {x.dtype}, {w_gate.dtype} and {w_up.dtype}")
