@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _OUT_DT, _changed, _empty_matrix, _require_cuda, _round_up, _stream_ptr
+from .ops import _INT8_MAX_K, _OUT_DT, _changed, _empty_matrix, _require_cuda, _round_up, _stream_ptr
 
 _ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH}
 
@@ -237,12 +237,14 @@ def gated_gemm(
     three or none) are one element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of the
     weights (``[1, F]`` / ``[F]``).  One kernel, ``g`` and ``u`` in fp32, one rounding to ``out_dtype`` (fp16, bf16 or
     fp32).  Weights are best column-major (a transposed view of ``[F, K]`` storage); row-major ones are re-laid out in
-    every call.  Up to 128 rows of ``x`` run in a kernel that streams the weights.  The result has no gradient; ``out``
+    every call.  ``K`` is at most 131056 for int8 operands.  Up to 128 rows of ``x`` run in a kernel that streams the weights.  The result has no gradient; ``out``
     must not overlap the inputs.
     """
     if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float8_e4m3fn, torch.int8):
         raise TypeError(f"gated_gemm expects three float8_e4m3fn or three int8 tensors, got {x.dtype}, {w_gate.dtype} and {w_up.dtype}")
     act = _check_gated(x, w_gate, w_up, activation, "gated_gemm")
+    if x.dtype == torch.int8 and x.shape[1] > _INT8_MAX_K:
+        raise ValueError(f"gated_gemm: K must be at most {_INT8_MAX_K} for int8 operands (the sums are int32), got {x.shape[1]}")
     if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TypeError(f"gated_gemm out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
     dev = _require_cuda(x, w_gate, w_up)

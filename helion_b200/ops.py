@@ -24,6 +24,8 @@ _OUT_DT = {
 }
 
 
+# The longest int8 products: 131072 of them may leave int32, and the kernels take K in multiples of 16.
+_INT8_MAX_K = 131072 - 16
 _TINY, _HUGE = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
@@ -204,7 +206,7 @@ def int8_gemm(
     The int8 sibling of :func:`fp8_gemm` with its arguments: ``scale_a`` / ``scale_b`` (fp32, both or neither) are one
     element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of ``y`` (``[1, N]`` / ``[N]``), as
     :func:`quantize_rows` and :func:`rms_norm_quantize` make them.  ``y`` is best column-major (a transposed view of
-    ``[N, K]`` storage); a row-major one is re-laid out in every call.  ``K`` is below 131072.  The result has no
+    ``[N, K]`` storage); a row-major one is re-laid out in every call.  ``K`` is at most 131056.  The result has no
     gradient; ``out`` must not overlap the inputs.
     """
     if x.dtype != torch.int8 or y.dtype != torch.int8:
@@ -214,6 +216,8 @@ def int8_gemm(
     m, k = x.shape
     k2, n = y.shape
     assert k == k2, f"size mismatch {k} != {k2}"
+    if k > _INT8_MAX_K:
+        raise ValueError(f"int8_gemm: K must be at most {_INT8_MAX_K} (the sums are int32), got {k}")
     if out_dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TypeError(f"int8_gemm out_dtype must be float16, bfloat16 or float32, got {out_dtype}")
     dev = _require_cuda(x, y)
