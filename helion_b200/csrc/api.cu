@@ -228,6 +228,10 @@ __global__ void wait_selftest_kernel(uint32_t* status, unsigned long long limit_
 
 using namespace hb;
 
+// Rows, columns and bytes of K that the GEMM kernels' 32-bit tile arithmetic takes: sizes and coordinates are rounded up to
+// tiles of at most 512.
+static constexpr int64_t kMaxTiled = (int64_t(1) << 31) - 512;
+
 static int ctx_error_code(int device) {
   return hb::device_init_error(device);
 }
@@ -346,8 +350,8 @@ static int fp8_gemm_impl(const void* x, const void* y, void* out, int64_t M, int
   if (out_dtype != HB200_DT_FP16 && out_dtype != HB200_DT_BF16 && out_dtype != HB200_DT_FP32) {
     return set_error(HB200_ERR_BAD_DTYPE, "fp8_gemm: out_dtype must be FP16, BF16 or FP32");
   }
-  if (M < 1 || N < 1 || K < 1 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) {
-    return set_error(HB200_ERR_BAD_SHAPE, "fp8_gemm: M, N, K must be in [1, 2^31)");
+  if (M < 1 || N < 1 || K < 1 || M > kMaxTiled || N > kMaxTiled || K > kMaxTiled) {
+    return set_error(HB200_ERR_BAD_SHAPE, "fp8_gemm: M, N, K must be in [1, 2^31 - 512]");
   }
   if (K % 16 != 0) return set_error(HB200_ERR_BAD_SHAPE, "fp8_gemm: K must be a multiple of 16");
   if (N % 8 != 0) return set_error(HB200_ERR_BAD_SHAPE, "fp8_gemm: N must be a multiple of 8");
@@ -435,8 +439,8 @@ int hb200_int8_gemm(const void* x, const void* y, void* out, int64_t M, int64_t 
   if (out_dtype != HB200_DT_FP16 && out_dtype != HB200_DT_BF16 && out_dtype != HB200_DT_FP32) {
     return set_error(HB200_ERR_BAD_DTYPE, "int8_gemm: out_dtype must be FP16, BF16 or FP32");
   }
-  if (M < 1 || N < 1 || K < 1 || M > INT32_MAX || N > INT32_MAX) {
-    return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: M and N must be in [1, 2^31), K positive");
+  if (M < 1 || N < 1 || K < 1 || M > kMaxTiled || N > kMaxTiled) {
+    return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: M and N must be in [1, 2^31 - 512], K positive");
   }
   if (K >= 131072) return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: K must be below 131072 (the sums are int32)");
   if (K % 16 != 0) return set_error(HB200_ERR_BAD_SHAPE, "int8_gemm: K must be a multiple of 16");
@@ -492,8 +496,8 @@ int hb200_gemm_16bit(const void* x, const void* y, void* out, int64_t M, int64_t
   if (out_dtype != in_dtype && out_dtype != HB200_DT_FP32) {
     return set_error(HB200_ERR_BAD_DTYPE, "gemm_16bit: out_dtype must be the operands' dtype or FP32");
   }
-  if (M < 1 || N < 1 || K < 1 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX / 2) {
-    return set_error(HB200_ERR_BAD_SHAPE, "gemm_16bit: M, N must be in [1, 2^31) and K in [1, 2^30)");
+  if (M < 1 || N < 1 || K < 1 || M > kMaxTiled || N > kMaxTiled || K > kMaxTiled / 2) {
+    return set_error(HB200_ERR_BAD_SHAPE, "gemm_16bit: M, N must be in [1, 2^31 - 512] and K in [1, 2^30 - 256]");
   }
   if (K % 8 != 0) return set_error(HB200_ERR_BAD_SHAPE, "gemm_16bit: K must be a multiple of 8");
   if (N % 8 != 0) return set_error(HB200_ERR_BAD_SHAPE, "gemm_16bit: N must be a multiple of 8");
@@ -555,8 +559,8 @@ static int gated_check(const char* what, int64_t M, int64_t F, int64_t K, int64_
                        int64_t up_rs, int64_t up_cs, int in_dtype, bool* w_colmajor, int64_t ldb[2]) {
   const std::string name(what);
   const int64_t per16 = in_dtype == HB200_DT_FP16 || in_dtype == HB200_DT_BF16 ? 8 : 16;  // elements in 16 bytes
-  if (M < 1 || F < 1 || K < 1 || M > INT32_MAX || F > INT32_MAX / 2 || K > INT32_MAX / 4) {
-    return set_error(HB200_ERR_BAD_SHAPE, name + ": M must be in [1, 2^31), F in [1, 2^30), K in [1, 2^29)");
+  if (M < 1 || F < 1 || K < 1 || M > kMaxTiled || F > kMaxTiled / 2 - 256 || K > INT32_MAX / 4) {
+    return set_error(HB200_ERR_BAD_SHAPE, name + ": M must be in [1, 2^31 - 512], F in [1, 2^30 - 512], K in [1, 2^29)");
   }
   if (K % per16 != 0) return set_error(HB200_ERR_BAD_SHAPE, name + ": K must be a multiple of 16 bytes");
   if (F % 8 != 0) return set_error(HB200_ERR_BAD_SHAPE, name + ": F must be a multiple of 8");
@@ -793,8 +797,8 @@ int hb200_fp8_gemm_splitk_static(const void* x, const void* y, void* out, int64_
   if (out_dtype != HB200_DT_FP16 && out_dtype != HB200_DT_BF16 && out_dtype != HB200_DT_FP32) {
     return set_error(HB200_ERR_BAD_DTYPE, "fp8_gemm_splitk_static: out_dtype must be FP16, BF16 or FP32");
   }
-  if (M < 1 || N < 1 || K < 1 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) {
-    return set_error(HB200_ERR_BAD_SHAPE, "fp8_gemm_splitk_static: M, N, K must be in [1, 2^31)");
+  if (M < 1 || N < 1 || K < 1 || M > kMaxTiled || N > kMaxTiled || K > kMaxTiled) {
+    return set_error(HB200_ERR_BAD_SHAPE, "fp8_gemm_splitk_static: M, N, K must be in [1, 2^31 - 512]");
   }
   if (K % 16 != 0 || N % 8 != 0) {
     return set_error(HB200_ERR_BAD_SHAPE, "fp8_gemm_splitk_static: K must be a multiple of 16 and N of 8");

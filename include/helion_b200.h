@@ -64,7 +64,7 @@ extern "C" {
  *      y_rs % 16 == 0), pointer 16-byte aligned.
  *   out: row-major, out_rs in elements, rows 16-byte aligned; out_dtype one of FP16/BF16/FP32
  *      (FP16 is what the reference produces).
- *   K % 16 == 0, N % 8 == 0, M >= 1.
+ *   K % 16 == 0, N % 8 == 0, M >= 1; each at most 2^31 - 512.
  *   cfg_id: index into the tile-config table, or -1 to let the library choose from the table.
  *      Every row computes the same product in stream order, with one exception that is never chosen
  *      automatically: row 23 (few rows of x, for chains of launches) starts reading y before the kernel
@@ -100,7 +100,8 @@ HB200_API int hb200_fp8_gemm_scaled(const void* x, const void* y, void* out, int
  * one conversion to fp32 and the two fp32 multiplications of hb200_fp8_gemm_scaled.  The int8 sibling of the fp8 GEMM
  * (examples/fp8_gemm.py:29-57); the reference has none.
  *   x: int8, row-major, x_rs % 16 == 0;  y: int8, column-major (y_rs == 1), y_cs % 16 == 0; both 16-byte aligned.
- *   K % 16 == 0, K < 131072 (so that no sum leaves int32);  N % 8 == 0;  out: FP16 / BF16 / FP32, rows 16-byte aligned.
+ *   K % 16 == 0, K < 131072 (so that no sum leaves int32);  N % 8 == 0;  M and N at most 2^31 - 512;
+ *   out: FP16 / BF16 / FP32, rows 16-byte aligned.
  *   scale_mode HB200_SCALE_NONE (scale_a and scale_b are not read), _TENSOR or _ROWWISE.
  *   cfg_id: -1, or a row of the GEMM table without split-K and chain forms (0-10, 14-18, 21); -1 and row 18 run up to
  *   128 rows of x in a kernel of their own that streams y. */
@@ -219,7 +220,8 @@ HB200_API int hb200_fp8_attention_preprocess(const void* q, const void* k, const
  *   act: HB200_ACT_SILU, HB200_ACT_GELU (with the normal distribution function) or HB200_ACT_GELU_TANH.
  *   x: row-major, rows 16-byte aligned; w_gate, w_up [K,F]: both column-major or, 16-bit operands only, both row-major, the
  *     other axis's stride giving 16-byte aligned rows; out: row-major, rows 16-byte aligned.
- *   K a multiple of 16 bytes (16 or 8 elements), K < 131072 for INT8; F % 8 == 0.  Pointers 16-byte aligned.
+ *   K a multiple of 16 bytes (16 or 8 elements), K < 131072 for INT8; F % 8 == 0, F at most
+ *     2^30 - 512, M at most 2^31 - 512.  Pointers 16-byte aligned.
  *   saved_p, saved_a: NULL, or (16-bit operands) [M,F] contiguous floats each that receive u * act'(g) and act(g) for
  *     hb200_gated_gemm_backward.
  * The reference has no counterpart (its examples stop at one product with an epilogue, examples/matmul.py:26-56). */
@@ -245,8 +247,8 @@ HB200_API int hb200_gated_gemm_backward(const void* dh, const void* x, const voi
                                         int64_t gate_cs, int64_t up_rs, int64_t up_cs, int dtype, void* workspace,
                                         size_t workspace_bytes, int device, void* stream);
 
-/* Bytes of workspace hb200_gated_gemm_backward needs on the current device: dG and dU, their largest magnitudes, and partial sums of dx where few
- * rows and columns of it leave it to be split along F. */
+/* Bytes of workspace hb200_gated_gemm_backward needs on the current device: dG and dU, their largest magnitudes, and
+ * partial sums of dx where few rows and columns of it leave it to be split along F. */
 HB200_API size_t hb200_gated_gemm_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 
 /* Row-wise quantisation to 8 bits: for each row of x [M,N] one scale and N codes,

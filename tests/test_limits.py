@@ -1,8 +1,12 @@
-"""The largest sizes that the operators take: what lies beyond is refused before any work."""
+"""The largest sizes that the operators take: what lies beyond is refused before any work, in Python and at the C entry points."""
 from __future__ import annotations
 
 import pytest
 import torch
+
+from helion_b200 import _lib
+
+BEYOND = 2**31 - 511  # a tile of up to 512 rows that starts below this may end past 2**31
 
 
 def test_int8_operands_longer_than_their_sums_allow():
@@ -24,3 +28,21 @@ def test_int8_operands_longer_than_their_sums_allow():
     x, w = torch.cat([x.view(torch.uint8)] * 2, 1).view(torch.float8_e4m3fn), torch.cat([w.view(torch.uint8)] * 2).view(torch.float8_e4m3fn)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         hb.gated_gemm(x, w, w)
+
+
+@pytest.mark.parametrize("m,n", [(BEYOND, 64), (2**31 - 1, 64), (64, (BEYOND + 7) // 8 * 8), (64, 2**31 - 8)])
+def test_gemm_entry_points_refuse_tiles_past_31_bits(built_library, m, n):
+    lib = built_library
+    assert lib.hb200_int8_gemm(256, 512, 1024, m, n, 64, 64, 1, 1, 64, n, _lib.DT_BF16, None, None, 0, -1, 0, None) == _lib.ERR_BAD_SHAPE
+    assert "int8_gemm" in _lib.last_error()
+    assert lib.hb200_gemm_16bit(256, 512, 1024, m, n, 64, 64, 1, 1, 64, n, _lib.DT_BF16, _lib.DT_BF16, None, 0, -1, 0, None) == _lib.ERR_BAD_SHAPE
+    assert lib.hb200_fp8_gemm(256, 512, 1024, m, n, 64, 64, 1, 1, 64, n, _lib.DT_BF16, -1, None, 0, 0, None) == _lib.ERR_BAD_SHAPE
+
+
+@pytest.mark.parametrize("m,f", [(BEYOND, 64), (2**31 - 1, 64), (64, 2**30 - 504), (64, 2**30)])
+def test_gated_entry_points_refuse_tiles_past_31_bits(built_library, m, f):
+    lib = built_library
+    assert lib.hb200_gated_gemm(256, 512, 768, 1024, m, f, 64, 64, 1, 64, 1, 64, f, _lib.DT_BF16, _lib.DT_BF16, 0, None, None, None, 0, None, None, 0, None) == _lib.ERR_BAD_SHAPE
+    assert "gated_gemm" in _lib.last_error()
+    got = lib.hb200_gated_gemm_backward(256, 512, 768, 1024, 2048, 4096, 8192, 16384, 32768, m, f, 64, f, 64, 1, 64, 1, 64, _lib.DT_BF16, 65536, 1 << 60, 0, None)
+    assert got == _lib.ERR_BAD_SHAPE and "gated_gemm_backward" in _lib.last_error()
