@@ -565,13 +565,24 @@ FewRowsArgs few_rows_args(const GemmArgs& a) {
   return f;
 }
 
+// Asks the instance that launch_few_rows runs for these arguments, so that the two cannot disagree.
 int few_rows_splits(const FewRowsArgs& a, DeviceCtx* ctx, int* splits) {
   int64_t at_once = 0;
-  return choose_splits<KIND_S8, 256, false, HB200_DT_BF16>(a, ctx, splits, &at_once);
+  switch (a.out_dtype) {
+    case HB200_DT_FP16:
+      return choose_splits<KIND_S8, 256, false, HB200_DT_FP16>(a, ctx, splits, &at_once);
+    case HB200_DT_BF16:
+      return choose_splits<KIND_S8, 256, false, HB200_DT_BF16>(a, ctx, splits, &at_once);
+    default:
+      return choose_splits<KIND_S8, 256, false, HB200_DT_FP32>(a, ctx, splits, &at_once);
+  }
 }
 
 int launch_few_rows(const FewRowsArgs& a, DeviceCtx* ctx) {
-  if (!a.gated) return launch_few_rows_out<KIND_S8, false>(a, ctx);
+  if (!a.gated) {
+    if (a.kind != KIND_S8) return set_error(HB200_ERR_BAD_DTYPE, "few rows: one weight is built for int8 operands only");
+    return launch_few_rows_out<KIND_S8, false>(a, ctx);
+  }
   switch (a.kind) {
     case KIND_E4M3:
       return launch_few_rows_out<KIND_E4M3, true>(a, ctx);
