@@ -165,7 +165,9 @@ def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     view of ``[F, K]`` storage) or row-major, both in the same layout (else one is copied).  When a gradient is needed
     the forward pass also keeps two fp32 ``[M,F]`` tensors; the backward pass returns ``x``'s and the weights' gradients
     in their dtype, and is not differentiable itself.  It rounds ``dh * u * act'(g)`` and ``dh * act(g)`` to the operands'
-    dtype (in fp16 scaled so that their largest value fits) before the products that give the gradients.
+    dtype (in fp16 scaled so that their largest value fits) before the products that give the gradients, and computes
+    both weights' gradients where one is wanted.  Operands whose ``K`` or ``F`` is not a multiple of 8 are padded, that is
+    copied, in every call.
 
     Both passes can be captured into a CUDA graph, unless an eager graph over the same leaf tensors, made by this
     function on the default stream, is alive: a call under capture that needs gradients is refused then.  (Other eager
@@ -237,8 +239,9 @@ def gated_gemm(
     three or none) are one element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of the
     weights (``[1, F]`` / ``[F]``).  One kernel, ``g`` and ``u`` in fp32, one rounding to ``out_dtype`` (fp16, bf16 or
     fp32).  Weights are best column-major (a transposed view of ``[F, K]`` storage); row-major ones are re-laid out in
-    every call.  ``K`` is at most 131056 for int8 operands.  Up to 128 rows of ``x`` run in a kernel that streams the weights.  The result has no gradient; ``out``
-    must not overlap the inputs.
+    every call, and so is everything where ``K`` is not a multiple of 16 or ``F`` not one of 8.  ``K`` is at most 131056
+    for int8 operands.  Up to 128 rows of ``x`` run in a kernel that streams the weights.  The result has no gradient;
+    ``out`` has unit column stride and rows at multiples of 16 bytes, and must not overlap the inputs.
     """
     if not (x.dtype == w_gate.dtype == w_up.dtype) or x.dtype not in (torch.float8_e4m3fn, torch.int8):
         raise TypeError(f"gated_gemm expects three float8_e4m3fn or three int8 tensors, got {x.dtype}, {w_gate.dtype} and {w_up.dtype}")

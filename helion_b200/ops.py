@@ -206,8 +206,9 @@ def int8_gemm(
     The int8 sibling of :func:`fp8_gemm` with its arguments: ``scale_a`` / ``scale_b`` (fp32, both or neither) are one
     element each, or one for each row of ``x`` (``[M, 1]`` / ``[M]``) and each column of ``y`` (``[1, N]`` / ``[N]``), as
     :func:`quantize_rows` and :func:`rms_norm_quantize` make them.  ``y`` is best column-major (a transposed view of
-    ``[N, K]`` storage); a row-major one is re-laid out in every call.  ``K`` is at most 131056.  The result has no
-    gradient; ``out`` must not overlap the inputs.
+    ``[N, K]`` storage); a row-major one is re-laid out in every call, and so are both operands where ``K`` is not a
+    multiple of 16 or ``N`` not one of 8.  ``K`` is at most 131056.  The result has no gradient; ``out`` has unit column
+    stride and rows at multiples of 16 bytes, and must not overlap the inputs.
     """
     if x.dtype != torch.int8 or y.dtype != torch.int8:
         raise TypeError(f"int8_gemm expects int8 inputs, got {x.dtype} and {y.dtype}")
