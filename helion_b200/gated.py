@@ -136,25 +136,31 @@ class _GatedMatmul(torch.autograd.Function):
         return dx, dw_gate if want_gate else None, dw_up if want_up else None, None
 
 
-def _refuse_capture(*leaves: torch.Tensor) -> None:
-    """Refuses a capture that living eager graphs over the leaves among ``leaves`` would break.
+def _reachable(nodes) -> set:
+    """All nodes of the graphs below ``nodes``, these included."""
+    seen, todo = set(), list(nodes)
+    while todo:
+        node = todo.pop()
+        if node not in seen:
+            seen.add(node)
+            todo += [n for n, _ in node.next_functions if n is not None]
+    return seen
+
+
+def _refuse_capture(*inputs: torch.Tensor) -> None:
+    """Refuses a capture that living eager graphs over the leaves below ``inputs`` would break.
 
     Autograd ties a leaf's gradient accumulator to the stream it was made on for as long as any graph over that leaf
     lives.  A backward pass under capture then waits on that stream, which CUDA forbids for the default one: the capture
     would be lost in the middle of the backward pass.  So it is refused here, before anything is recorded.
     """
-    edges = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t.requires_grad and t.grad_fn is None]
-    seen, todo = set(), _eager_nodes.snapshot()
-    while todo:
-        node = todo.pop()
-        if any(node is e for e in edges):
-            raise RuntimeError(
-                "gated_matmul: an eager graph over the same leaf tensors, made on the default stream, is still alive; "
-                "a backward pass cannot be captured next to it. Drop its results first, or make it on another stream"
-            )
-        if node not in seen:
-            seen.add(node)
-            todo += [n for n, _ in node.next_functions if n is not None]
+    here = _reachable(torch.autograd.graph.get_gradient_edge(t).node for t in inputs if t.requires_grad)
+    # (both sets keep their nodes' Python objects, so that one node is one object in both)
+    if any(hasattr(n, "variable") for n in here & _reachable(_eager_nodes.snapshot())):
+        raise RuntimeError(
+            "gated_matmul: an eager graph over the same leaf tensors, made on the default stream, is still alive; "
+            "a backward pass cannot be captured next to it. Drop its results first, or make it on another stream"
+        )
 
 
 def gated_matmul(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation: str = "silu") -> torch.Tensor:
