@@ -430,8 +430,8 @@ __global__ void __launch_bounds__(1024) row_quantize_kernel(RowQuantArgs a) {
 // residual); values go to registers on arrival, and the reduction's barrier hands the stage back for the row `stages` ahead.
 //
 // Measured, bf16, a CTA a row / ring (us; % of the copy bandwidth of 6.55 TB/s): with norm and residual 8192 x 4096
-// 44.7 / 42.2 (85 %), 4096 x 8192 51.7 / 40.8, 4096 x 14336 93.3 / 68.8 (91 %), 600 x 8192 10.0 / 9.1, but 2048 x 4096
-// 12.7 / 14.0; quantised 8192 x 4096 27.6 / 21.6 (71 %), 4096 x 14336 36.3 / 32.5 (83 %), but 600 x 8192 4.1 / 5.5.
+// 44.5 / 42.3 (85 %), 4096 x 8192 52.4 / 41.0, 4096 x 14336 93.1 / 68.6 (91 %), 600 x 8192 10.9 / 10.4, but 2048 x 4096
+// 13.4 / 15.8; quantised 8192 x 4096 27.6 / 23.0 (67 %), 4096 x 14336 47.0 / 31.9 (84 %), but 600 x 8192 4.2 / 5.4.
 // With the norm alone, and for fp32 rows, whose CTAs hold twice the bytes each, it gains nothing (4096 x 8192 with norm
 // 29.7 / 32.0; fp32 4096 x 8192 with residual 70.3 / 77.5), nor for rows that are not aligned.
 // ------------------------------------------------------------------------------------------------
@@ -597,9 +597,9 @@ template <int SRC_DT, int MODE, int TIER>
 int launch_row_size(const RowQuantArgs& a, const RowQuantLaunch& l) {
   const int64_t groups = (a.N + (TIER == ROW_PHASED ? 7 : 0) + 7) / 8;  // a phase adds a group at most
   // CTAs of up to 1024 threads, rather than 512, where a row's own latency counts: rows that have an SM each (one row of
-  // 14336 bf16 with residual 4.6 / 3.6 us, quantised 2.5 / 2.2 us), and odd rows with a residual, whose masks and
-  // shifts are most of their time (1237 x 5003 15.5 / 14.7 us, 4096 x 4099 47.0 / 38.5 us).  Elsewhere the smaller ones hold
-  // more rows a SM (1237 x 8192 quantised 7.8 / 10.5 us).
+  // 14336 bf16 with residual 4.4 / 3.4 us, quantised 2.4 / 2.2 us), and odd rows with a residual, whose masks and
+  // shifts are most of their time (1237 x 5003 17.1 / 15.7 us, 4096 x 4099 47.6 / 39.2 us).  Elsewhere the smaller ones hold
+  // more rows a SM (1237 x 8192 quantised 8.0 / 10.5 us).
   const bool wide = l.M <= l.ctx->num_sms || (TIER == ROW_PHASED && MODE == 2 && groups <= 1024);
   const int vpt = groups <= (wide ? 1024 : 512) ? 1 : (groups <= (wide ? 2048 : 1024) ? 2 : 4);
   const int threads = static_cast<int>(std::min<int64_t>(((groups + vpt - 1) / vpt + 31) / 32 * 32, 1024));
