@@ -4,7 +4,7 @@
 //
 //   s = x + residual            (rounded to x's type in residual_out; the norm takes the unrounded fp32 sum)
 //   y = s * rstd * w,  rstd = 1 / sqrt(mean(s^2) + eps)          (quantize_rows: y = x)
-//   scale = max|y| / Q,  code = round(y / scale)                 Q = 448 (e4m3) or 127 (int8)
+//   scale = max|y| / Q,  code = round(y Q / max|y|)              Q = 448 (e4m3) or 127 (int8)
 //
 // rstd is one factor for the whole row, so max|y| = rstd * max|s w| and code = (s w) * (Q / max|s w|): the sum of
 // squares and the largest magnitude come out of ONE pass and one block reduction, and rstd does not enter the

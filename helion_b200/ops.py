@@ -492,8 +492,8 @@ def quantize_rows(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``[..., N]`` -> 8-bit codes ``[..., N]`` and one fp32 scale for each row ``[..., 1]``, ``x ~ codes * scales``.
 
-    ``scale = max|x| / Q`` and ``code = round(x / scale)`` in fp32 with ``Q`` = 448 (``float8_e4m3fn``) or 127
-    (``int8``): what :func:`fp8_gemm`, :func:`int8_gemm` and :func:`gated_gemm` take as ``x`` and its row scale.
+    ``scale = max|x| / Q`` and ``code = round(x * Q / max|x|)``, exact ties to even, with ``Q`` = 448 (``float8_e4m3fn``)
+    or 127 (``int8``): what :func:`fp8_gemm`, :func:`int8_gemm` and :func:`gated_gemm` take as ``x`` and its row scale.
     ``x`` is fp16, bf16 or fp32.  A row of zeros (``max|x| < 2**-100``) gets zero codes and the smallest normal
     scale; a NaN makes its row's scale NaN, an infinity makes it infinite.  ``out`` and ``scale_out`` (contiguous, apart
     from ``x``) take the results of a caller that keeps its buffers.  The results have no gradient.

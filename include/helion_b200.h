@@ -252,8 +252,8 @@ HB200_API int hb200_gated_gemm_backward(const void* dh, const void* x, const voi
 HB200_API size_t hb200_gated_gemm_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 
 /* Row-wise quantisation to 8 bits: for each row of x [M,N] one scale and N codes,
- *   scale = max(max|x| / Q, FLT_MIN),  code = round_to_nearest_even(x / scale),  Q = 448 (E4M3) or 127 (INT8),
- * in fp32.  The codes and scales are what hb200_fp8_gemm_scaled / hb200_int8_gemm take as x and scale_a with
+ *   scale = max(max|x| / Q, FLT_MIN),  code = round_to_nearest_even(x * Q / max|x|),  Q = 448 (E4M3) or 127 (INT8),
+ * the quotient within 2^-46 before one rounding to fp32, so that exact ties are seen as such.  The codes and scales are what hb200_fp8_gemm_scaled / hb200_int8_gemm take as x and scale_a with
  * HB200_SCALE_ROWWISE.  The reference has no counterpart (its fp8 example casts without scales,
  * examples/fp8_gemm.py:60-75).
  *   x: src_dtype FP16, BF16 or FP32, row stride x_rs >= N elements, aligned to its element size;
